@@ -72,6 +72,14 @@ typedef enum vx_index_kind {
   VX_KIND_PQ = 8       /* QuantizerKind.PQ -> QuantizedFlatScanAdapter(PQVectors) */
 } vx_index_kind;
 
+/* Element types of the 8-bit row functions' buffers. */
+typedef enum vx_dtype {
+  VX_F32 = 0,
+  VX_F16 = 1,
+  VX_BF16 = 2,
+  VX_E4M3 = 3 /* stored rows: e4m3 codes with scale exponents (vx_fp8_write_device) */
+} vx_dtype;
+
 typedef struct vx_index vx_index;
 
 /* ---- library ------------------------------------------------------------------------ */
@@ -339,6 +347,60 @@ VX_API int vx_merge_shards_device(int32_t device, int32_t nshards, const int64_t
                            const int32_t* d_shard_ids, const float* d_shard_scores,
                            const int32_t* d_shard_counts, int32_t kin, int32_t nq, int32_t k,
                            int32_t* d_ids, float* d_scores, int32_t* d_counts, void* stream);
+
+/* ---- 8-bit float rows ------------------------------------------------------------------
+ * No counterpart in the reference, whose quantizers are integer or binary.  Rows are kept as e4m3
+ * codes with one power-of-two scale for each block of 128 dimensions, in two device buffers that
+ * the caller owns (and may slice by rows, save or copy):
+ *   codes  [capacity][code_pitch]   e4m3; code_pitch = dim rounded up to 128, columns >= dim zero;
+ *                                   16-byte aligned
+ *   scales [capacity][scale_pitch]  byte b of block j = 2^(b - 127), 255 = NaN; scale_pitch =
+ *                                   code_pitch / 128 rounded up to 4; 4-byte aligned
+ * (vx_fp8_pitch gives both).  A block's exponent is the smallest e >= -127 with max |x| <= 448 * 2^e
+ * and a code the nearest e4m3 value of x / 2^e, ties to even: |error| <= 2^-4 |x| or 2^-10 * 2^e,
+ * whichever is larger.  A block with a NaN or an infinity becomes NaN throughout.  dim <= 65536,
+ * capacity < 2^31.  Buffers are device memory of `device`; calls are queued on `stream`, allocate only
+ * stream-ordered scratch and can be captured into a graph.  Calls on one store that write and read the
+ * same rows must be ordered by the caller (one stream, or events). */
+VX_API int vx_fp8_pitch(int32_t dim, int32_t* code_pitch, int32_t* scale_pitch);
+/* Quantises rows [n][dim] (type VX_F32 / VX_F16 / VX_BF16, row_stride elements apart) into the store:
+ * row i goes to slots[i] (slot_bytes 4 or 8: int32 or int64), or to first + i when slots is NULL
+ * (first + n <= capacity).  A slot outside [0, capacity) skips its row; where rows of a call name the
+ * same slot, the last of them is kept.  Other slots are left as they are. */
+VX_API int vx_fp8_write_device(int32_t device, const void* rows, int32_t type, int64_t n, int32_t dim,
+                               int64_t row_stride, const void* slots, int32_t slot_bytes, int64_t first,
+                               uint8_t* codes, uint8_t* scales, int64_t capacity, void* stream);
+/* Reads n stored rows back as out [n][dim] (type VX_F32 / VX_F16 / VX_BF16, out_stride elements apart):
+ * the rows of slots (slot_bytes 4 or 8, e.g. the ordinals of a search), or first .. first + n - 1 when
+ * slots is NULL.  Values are exact in fp32, rounded once to fp16 / bf16; a slot outside [0, capacity)
+ * reads as zeros (a search's unused tail holds ordinal -1). */
+VX_API int vx_fp8_read_device(int32_t device, const uint8_t* codes, const uint8_t* scales, int64_t capacity,
+                              int32_t dim, const void* slots, int32_t slot_bytes, int64_t first, int64_t n, void* out,
+                              int32_t out_type, int64_t out_stride, void* stream);
+/* out[i][j] = dot(query i, stored row j) for every query and each of the n stored rows, out [nq][n]
+ * out_stride elements apart, out_type VX_F32 / VX_F16 / VX_BF16.  Queries [nq][dim] of VX_F32 / VX_F16 /
+ * VX_BF16, query_stride elements apart, are quantised as vx_fp8_write_device does; or they are stored
+ * rows: query_type VX_E4M3 with their codes and query_scales (query_stride is not used).  Products are
+ * exact and summed in fp32; a NaN block makes its query's or row's results NaN. */
+VX_API int vx_fp8_scores_device(int32_t device, const void* queries, int32_t query_type, const uint8_t* query_scales,
+                                int64_t nq, int64_t query_stride, const uint8_t* codes, const uint8_t* scales,
+                                int64_t n, int32_t dim, void* out, int32_t out_type, int64_t out_stride, void* stream);
+/* The products of `groups` groups: queries query_offsets[g] .. query_offsets[g + 1] - 1 against stored rows
+ * row_offsets[g] .. row_offsets[g + 1] - 1 (device arrays [groups + 1], int64), e.g. (query, list) pairs
+ * sorted by list and the lists' rows, or tokens sorted by expert and the experts' weights.
+ * out[i][j - row_offsets[g]] for query i of group g, out [nq][max_rows] out_stride elements apart; results
+ * past a group's rows, and rows of out in no group, are left as they are; a group's rows past max_rows are
+ * not scored.  Offsets are clamped to the operands' sizes and an end below its start is an empty
+ * group, so no offsets read or write out of range; groups whose queries overlap write the same results. */
+VX_API int vx_fp8_scores_grouped_device(int32_t device, const void* queries, int32_t query_type,
+                                        const uint8_t* query_scales, int64_t nq, int64_t query_stride,
+                                        const int64_t* query_offsets, const uint8_t* codes, const uint8_t* scales,
+                                        int64_t n, const int64_t* row_offsets, int64_t groups, int32_t dim, void* out,
+                                        int32_t out_type, int64_t out_stride, int64_t max_rows, void* stream);
+/* Waits for `stream` and reports whether a bounded device-side wait of a vx_fp8_scores* call on
+ * `device` has run out since the last report (VX_ERR_DEVICE_TIMEOUT; that call's results are
+ * incomplete).  The next vx_fp8_scores* call on the device reports it too, without waiting. */
+VX_API int vx_fp8_check(int32_t device, void* stream);
 
 #ifdef __cplusplus
 }

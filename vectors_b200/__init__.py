@@ -5,6 +5,15 @@ list scan) run as hand-written CUDA kernels in ``libvx.so``; this package is the
 mirror of the reference's index SPI over that library's C ABI (include/vx.h).
 """
 from ._native import VxError, device_count, kernel_launches, lib  # noqa: F401
+from .fp8 import (  # noqa: F401
+    fp8_check,
+    fp8_empty,
+    fp8_pitch,
+    fp8_read_device,
+    fp8_scores_device,
+    fp8_scores_grouped_device,
+    fp8_write_device,
+)
 from .index_spi import (  # noqa: F401
     FlatScanAdapter,
     GpuUnavailableException,
@@ -41,6 +50,13 @@ __all__ = [
     "ivf_graph_info",
     "merge_shards_device",
     "shard_offsets",
+    "fp8_check",
+    "fp8_empty",
+    "fp8_pitch",
+    "fp8_read_device",
+    "fp8_scores_device",
+    "fp8_scores_grouped_device",
+    "fp8_write_device",
     "device_count",
     "kernel_launches",
     "lib",

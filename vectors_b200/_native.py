@@ -24,6 +24,8 @@ VX_ERR_FORMAT = 8
 
 VX_KIND_FLAT, VX_KIND_FP16, VX_KIND_SQ8, VX_KIND_BQ, VX_KIND_IVFPQ, VX_KIND_IVFFLAT, VX_KIND_SQ4, VX_KIND_BBQ, VX_KIND_PQ = range(9)
 
+VX_F32, VX_F16, VX_BF16, VX_E4M3 = range(4)
+
 _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
@@ -70,6 +72,12 @@ SIGNATURES = {
     "vx_ivfflat_scan_pairs_device": [_P, _P, _I32, _I32, _I32, _I32, _P, _P, _P, _P],
     "vx_ivfflat_merge_pairs_device": [_P, _I32, _I32, _I32, _P, _P, _P, _P, _F32, _P, _P, _P, _P],
     "vx_merge_shards_device": [_I32, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _P],
+    "vx_fp8_pitch": [_I32, _P, _P],
+    "vx_fp8_write_device": [_I32, _P, _I32, _I64, _I32, _I64, _P, _I32, _I64, _P, _P, _I64, _P],
+    "vx_fp8_read_device": [_I32, _P, _P, _I64, _I32, _P, _I32, _I64, _I64, _P, _I32, _I64, _P],
+    "vx_fp8_scores_device": [_I32, _P, _I32, _P, _I64, _I64, _P, _P, _I64, _I32, _P, _I32, _I64, _P],
+    "vx_fp8_scores_grouped_device": [_I32, _P, _I32, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I32, _P, _I32, _I64, _I64, _P],
+    "vx_fp8_check": [_I32, _P],
     "vx_bq_scan_candidates_noalloc": [_P, _P, _I32, _I32, _I32, _P, _P, _P, _P],
 }
 

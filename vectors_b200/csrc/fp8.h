@@ -1,0 +1,93 @@
+// fp8.h -- rows kept as e4m3 codes with one power-of-two scale per block of 128 dimensions:
+// quantising rows into a store, reading them back, and the score products on them (fp8.cu,
+// fp8_scores.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace vx {
+
+constexpr int kFp8Block = 128;        // dimensions that share a scale
+constexpr int kFp8MaxDim = 1 << 16;
+constexpr int kFp8MaxWidth = 224;     // queries of one product tile (TMEM columns per accumulator)
+// batches of at most this many rows find repeated slots by comparing slots directly (fp8.cu)
+constexpr int64_t kFp8DirectSlots = 256;
+
+inline int fp8_blocks(int dim) { return (dim + kFp8Block - 1) / kFp8Block; }
+inline int fp8_code_pitch(int dim) { return fp8_blocks(dim) * kFp8Block; }  // bytes of codes per row
+inline int fp8_scale_pitch(int dim) { return (fp8_blocks(dim) + 3) / 4 * 4; }  // bytes of scales per row
+
+struct Fp8WriteArgs {
+  const void* rows;  // [n] rows, `stride` elements apart
+  int type;          // vx_dtype of the rows
+  int64_t n;
+  int dim;
+  int64_t stride;
+  const void* slots;  // destination of each row, or null: first, first + 1, ...
+  int slot_bytes;     // 4 or 8
+  int64_t first;
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t capacity;
+  int32_t* owner;  // [capacity] scratch; needed for more than kFp8DirectSlots rows with slots
+};
+
+struct Fp8ReadArgs {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int64_t capacity;
+  int dim;
+  const void* slots;
+  int slot_bytes;
+  int64_t first, n;
+  void* out;
+  int type;
+  int64_t stride;
+};
+
+// `early`: the kernel lets a dependent launch begin before it ends.
+cudaError_t launch_fp8_write(const Fp8WriteArgs& a, bool early, int* launches, cudaStream_t st);
+cudaError_t launch_fp8_read(const Fp8ReadArgs& a, cudaStream_t st);
+
+struct Fp8ScoreArgs {
+  const uint8_t* row_scales;
+  int64_t nrows;
+  const uint8_t* query_scales;
+  int64_t nq;
+  int scale_words;  // 32-bit scale words per row
+  int kchunks;      // 128-byte chunks of a row
+  void* out;
+  int64_t ldo;  // elements between two queries' results
+  // one group of every row and query: row_off null
+  const int64_t* row_off;    // [groups + 1]
+  const int64_t* query_off;  // [groups + 1]
+  const int64_t* tile_off;   // [groups + 1], from launch_fp8_group_tiles
+  int64_t groups;
+  int64_t max_cols;  // results kept per query (groups with more rows are cut there)
+  uint64_t timeout_ns;
+  int32_t* err;
+  // filled in by launch_fp8_scores
+  int64_t tiles;
+  int query_tiles;
+  int width;
+  int stages;
+  int wait_first;
+};
+
+// The operands' tensor maps: `rows` with 128-row boxes, queries[i] with boxes of 64 >> i rows.
+struct Fp8Maps {
+  CUtensorMap rows;
+  CUtensorMap queries[3];
+};
+
+// Tiles before each group, from untrusted offsets (clamped to the operands' sizes).
+cudaError_t launch_fp8_group_tiles(const int64_t* row_off, const int64_t* query_off, int64_t groups, int64_t nrows,
+                                   int64_t nq, int64_t max_cols, int64_t* tile_off, cudaStream_t st);
+// after_prep: the launch before this one on `st` is a kernel of this file's that encoded the
+// queries or counted the groups' tiles; this launch may begin before that one ends.
+cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& a, int out_type, int num_sms, bool after_prep,
+                              cudaStream_t st);
+
+}  // namespace vx

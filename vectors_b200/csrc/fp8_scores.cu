@@ -1,0 +1,504 @@
+// fp8_scores.cu -- score products on 8-bit rows: S[i][j] = sum over 128-dim blocks b of
+// 2^(eq[i][b] + er[j][b]) * sum_k q[i][k] r[j][k], for one group of all rows and queries or for
+// many groups of different sizes (each group's queries against its own rows).
+//
+// Tensor cores.  tcgen05 block scaling (kind::mxf8f6f4) multiplies e4m3 operands and applies the
+// two power-of-two scales inside the instruction, for every 32 elements of K; a block of 128 is four
+// instructions with the same scales.  The whole sum over K stays in the fp32 accumulator in TMEM,
+// and no scale passes through the epilogue.  (With arbitrary fp32 scales each 128-element partial
+// sum would have to be read from TMEM and multiplied in the FP32 pipe, which takes as long as the
+// MMAs themselves.)
+//
+// Tiling.  2-CTA clusters (cta_group::2), 256 stored rows x up to 224 queries.  The stored rows are
+// the MMA's M operand, so a TMEM lane holds one stored row and an epilogue warp writes 32
+// consecutive results of one query at a time: coalesced, with no transposition.  The queries are
+// its N operand, any multiple of 32, so few queries cost few MMA cycles and the kernel then streams
+// the stored rows at HBM speed; each CTA stages its 128 rows and half the queries of a 128-byte K
+// chunk by TMA (128-byte swizzle).  224 and not 256 queries: two accumulators take 448 of the 512
+// TMEM columns and leave 60 for a ring of five scale slots.
+//
+// Scales.  A slot holds the scale words of four K chunks (512 dimensions): 4 columns for the CTA's
+// 128 rows and 8 for the queries.  A stored row's scale bytes are consecutive, so a 32-bit load
+// gives four chunks' exponents, which go to TMEM as they are (the descriptor's scale id picks the
+// byte).  Four warps per CTA, one for each TMEM lane quarter, load and store them.
+//
+// Warps: 0 TMA, 1 TMEM and (leader CTA) MMA, 2-5 epilogue, 6-9 scales.  Every wait is bounded; on
+// expiry the error word is set, the roles unwind and TMEM is released.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/vx.h"
+#include "fp8.h"
+#include "sm100.cuh"
+
+namespace vx {
+namespace {
+
+using namespace sm100;
+
+constexpr int kThreads = 320;
+constexpr int kTmemCols = 512;
+constexpr int kRowBytes = 128 * 128;  // a CTA's stored-row operand per stage
+constexpr int kScaleSlots = 5;
+constexpr int kSlotCols = 12;
+constexpr uint32_t kScaleBase = 2 * kFp8MaxWidth;
+constexpr size_t kMaxSmem = 232448;
+constexpr size_t kBarrierBytes = 512;
+constexpr int kMaxStages = 12;
+
+static_assert(kScaleBase + kScaleSlots * kSlotCols <= kTmemCols, "TMEM columns");
+
+__host__ __device__ constexpr size_t stage_bytes(int width) { return kRowBytes + (size_t)width / 2 * 128; }
+
+// One tile: rows [row, row + rows) against queries [query, query + queries).
+struct Tile {
+  int64_t row, query;
+  int64_t col;  // column of the first row's results
+  int rows, queries;
+  int width;    // MMA N: queries rounded up to 32
+};
+
+__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t hi) { return v < 0 ? 0 : v > hi ? hi : v; }
+
+// A group's rows and queries from its (untrusted) offsets.
+struct Group {
+  int64_t row0, nrows, query0, nqueries;
+  int64_t query_tiles, tiles;
+  int width;
+};
+__device__ __forceinline__ Group group_of(const int64_t* row_off, const int64_t* query_off, int64_t g, int64_t nrows,
+                                          int64_t nq, int64_t max_cols) {
+  Group r;
+  r.row0 = clamp64(row_off[g], nrows);
+  r.nrows = clamp64(clamp64(row_off[g + 1], nrows) - r.row0, max_cols);
+  r.query0 = clamp64(query_off[g], nq);
+  r.nqueries = clamp64(clamp64(query_off[g + 1], nq) - r.query0, nq);
+  r.query_tiles = (r.nqueries + kFp8MaxWidth - 1) / kFp8MaxWidth;
+  r.width = r.query_tiles ? (int)(((r.nqueries + r.query_tiles - 1) / r.query_tiles + 31) / 32 * 32) : 32;
+  r.tiles = (r.nrows + 255) / 256 * r.query_tiles;
+  return r;
+}
+
+// Walks a work unit's tiles in order.  One group: tile t is (row tile t / query_tiles, query tile
+// t % query_tiles).  Several: the group of the unit's first tile by bisection of tile_off, later ones
+// by stepping.
+struct Walk {
+  const Fp8ScoreArgs& a;
+  Group g;
+  int64_t group;  // current group (groups only)
+  int64_t base;   // tiles before it
+  __device__ __forceinline__ Walk(const Fp8ScoreArgs& args, int64_t first) : a(args), group(0), base(0) {
+    if (!a.row_off) {
+      g.row0 = g.query0 = 0;
+      g.nrows = a.nrows;
+      g.nqueries = a.nq;
+      g.query_tiles = a.query_tiles;
+      g.width = a.width;
+      return;
+    }
+    int64_t lo = 0, hi = a.groups;  // tile_off[lo] <= first < tile_off[hi]
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.tile_off[mid] <= first) lo = mid;
+      else hi = mid;
+    }
+    group = lo;
+    base = a.tile_off[lo];
+    g = group_of(a.row_off, a.query_off, lo, a.nrows, a.nq, a.max_cols);
+  }
+  __device__ __forceinline__ Tile at(int64_t p) {
+    if (a.row_off) {
+      while (p >= base + g.tiles && group + 1 < a.groups) {
+        base += g.tiles;
+        group++;
+        g = group_of(a.row_off, a.query_off, group, a.nrows, a.nq, a.max_cols);
+      }
+    }
+    const int64_t t = p - base;
+    const int64_t rt = t / g.query_tiles, qt = t % g.query_tiles;
+    Tile x;
+    x.row = g.row0 + rt * 256;
+    x.col = a.row_off ? rt * 256 : x.row;
+    const int64_t rl = g.nrows - rt * 256;
+    x.rows = rl < 256 ? (int)rl : 256;
+    x.query = g.query0 + qt * g.width;
+    const int64_t ql = g.nqueries - qt * g.width;
+    x.queries = ql < g.width ? (int)(ql < 0 ? 0 : ql) : g.width;
+    x.width = x.queries > 0 ? (x.queries + 31) / 32 * 32 : 32;
+    return x;
+  }
+};
+
+template <int kType>
+struct Out;
+template <>
+struct Out<VX_F32> {
+  using T = float;
+  static __device__ __forceinline__ T of(uint32_t v) { return __uint_as_float(v); }
+};
+template <>
+struct Out<VX_F16> {
+  using T = __half;
+  static __device__ __forceinline__ T of(uint32_t v) { return __float2half_rn(__uint_as_float(v)); }
+};
+template <>
+struct Out<VX_BF16> {
+  using T = __nv_bfloat16;
+  static __device__ __forceinline__ T of(uint32_t v) { return __float2bfloat16_rn(__uint_as_float(v)); }
+};
+
+template <int kType>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_scores_kernel(const __grid_constant__ Fp8Maps maps, const __grid_constant__ Fp8ScoreArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int n_stages = a.stages;
+  const size_t stage_size = stage_bytes(a.width);
+  uint64_t* full = (uint64_t*)(stages + n_stages * stage_size);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* sfull = empty + kMaxStages;
+  uint64_t* sempty = sfull + kScaleSlots;
+  uint64_t* tfull = sempty + kScaleSlots;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drained = tempty + 2;
+  uint32_t* tmem_slot = (uint32_t*)(drained + 1);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < n_stages; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < kScaleSlots; s++) {
+      mbar_init(&sfull[s], 8);  // four scale warps of each CTA
+      mbar_init(&sempty[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 8);  // four epilogue warps of each CTA
+    }
+    mbar_init(drained, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // The launch before this one wrote the encoded queries, the groups' tile counts or both.
+  if (a.wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int64_t total = a.row_off ? a.tile_off[a.groups] : a.tiles;
+  const int64_t p0 = total * unit / units, p1 = total * (unit + 1) / units;
+
+  auto give_up = [&]() {
+    *abort_flag = 1;
+    record_error(a.err, kDevWaitTimeout);
+  };
+
+  if (warp == 0) {
+    if (lane == 0 && p0 < p1) {
+      prefetch_tmap(&maps.rows);
+      for (int i = 0; i < 3; i++) prefetch_tmap(&maps.queries[i]);
+      const uint64_t pol_q = policy_evict_last();  // query tiles are read again for every row tile
+      const uint64_t pol_r = policy_evict_normal();
+      const uint32_t full0 = mapa_shared(smem_addr(&full[0]), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      Walk walk(a, p0);
+      for (int64_t p = p0; p < p1 && !*abort_flag; p++) {
+        const Tile t = walk.at(p);
+        const int half = t.width >> 1;  // query rows of this CTA
+        const int32_t yr = (int32_t)t.row + (int)rank * 128;
+        const int32_t yq = (int32_t)t.query + (int)rank * half;
+        for (int kc = 0; kc < a.kchunks; kc++) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, a.timeout_ns, abort_flag)) {
+            give_up();
+            break;
+          }
+          uint8_t* s = stages + stage * stage_size;
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2u * (uint32_t)stage_bytes(t.width));
+          const uint32_t bar = full0 + (uint32_t)(stage * 8);
+          tma_load_2d_pair(s, &maps.rows, bar, kc * 128, yr, pol_r);
+          s += kRowBytes;
+          int32_t y = yq;
+#pragma unroll
+          for (int i = 0; i < 3; i++) {  // the half's rows as boxes of 64, 32 and 16
+            const int box = 64 >> i;
+            if (half & box) {
+              tma_load_2d_pair(s, &maps.queries[i], bar, kc * 128, y, pol_q);
+              s += box * 128;
+              y += box;
+            }
+          }
+          if (++stage == n_stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (*abort_flag) {
+        // Let the loads already issued land before the cluster's shared memory is released.
+        const uint64_t until = globaltimer_ns() + 2000000ull;
+        while (globaltimer_ns() < until) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader && p0 < p1) {
+      int stage = 0, slot = 0;
+      uint32_t phase = 0, sphase = 0;
+      Walk walk(a, p0);
+      for (int64_t p = p0; p < p1 && !*abort_flag; p++) {
+        const Tile t = walk.at(p);
+        const int64_t li = p - p0;
+        const int acc = (int)(li & 1);
+        if (!mbar_wait(&tempty[acc], (uint32_t)((li >> 1) & 1) ^ 1u, a.timeout_ns, abort_flag)) {
+          give_up();
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + (uint32_t)(acc * kFp8MaxWidth);
+        const uint32_t idesc0 = idesc_mxf8(256, t.width, 0);
+        bool ok = true;
+        for (int kc = 0; kc < a.kchunks; kc++) {
+          const int sub = kc & 3;
+          if (sub == 0 && !mbar_wait(&sfull[slot], sphase, a.timeout_ns, abort_flag)) ok = false;
+          if (ok && !mbar_wait(&full[stage], phase, a.timeout_ns, abort_flag)) ok = false;
+          if (!ok) {
+            give_up();
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_addr(stages + stage * stage_size);
+          const uint64_t da = sw128_kmajor_desc(sa), db = sw128_kmajor_desc(sa + kRowBytes);
+          const uint32_t scales = tmem_base + kScaleBase + (uint32_t)(slot * kSlotCols);
+          const uint32_t idesc = idesc0 | ((uint32_t)sub << 4) | ((uint32_t)sub << 29);
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++)
+            mma_mxf8_pair(d, da + 2ull * kk, db + 2ull * kk, idesc, scales, scales + 4, (kc | kk) != 0 ? 1u : 0u);
+          mma_commit_pair_mc(&empty[stage], (uint16_t)0x3);
+          if (++stage == n_stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (sub == 3 || kc + 1 == a.kchunks) {
+            mma_commit_pair_mc(&sempty[slot], (uint16_t)0x3);
+            if (++slot == kScaleSlots) {
+              slot = 0;
+              sphase ^= 1u;
+            }
+          }
+        }
+        if (!ok) break;
+        mma_commit_pair_mc(&tfull[acc], (uint16_t)0x3);
+      }
+      if (*abort_flag) {  // MMAs in flight end before their TMEM and shared memory are released
+        mma_commit_pair_mc(drained, (uint16_t)0x1);
+        const uint64_t until = globaltimer_ns() + 2000000ull;
+        while (!mbar_try_wait(drained, 0) && globaltimer_ns() < until) {
+        }
+      }
+    }
+  } else if (warp < 6) {
+    // ---------------- epilogue: one stored row per lane, one query per TMEM column
+    using T = typename Out<kType>::T;
+    const int quarter = warp & 3;
+    const int my_row = (int)rank * 128 + quarter * 32 + lane;
+    const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0);
+    if (p0 < p1) {
+      Walk walk(a, p0);
+      for (int64_t p = p0; p < p1; p++) {
+        const Tile t = walk.at(p);
+        const int64_t li = p - p0;
+        const int acc = (int)(li & 1);
+        const bool row_in = my_row < t.rows;
+        T* out = (T*)a.out + t.query * a.ldo + t.col + my_row;
+        if (__shfl_sync(0xFFFFFFFFu, *abort_flag, 0)) break;
+        const bool ok = mbar_wait(&tfull[acc], (uint32_t)((li >> 1) & 1), a.timeout_ns, abort_flag);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          if (lane == 0) give_up();
+          break;
+        }
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * kFp8MaxWidth);
+        for (int c0 = 0; c0 < t.queries; c0 += 32) {
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(taddr + (uint32_t)c0, v);
+          tmem_ld_wait_v(v);
+          const int lim = t.queries - c0;
+          if (row_in) {
+            T* o = out + c0 * a.ldo;
+            if (lim >= 32) {
+#pragma unroll
+              for (int j = 0; j < 32; j++) {
+                *o = Out<kType>::of(v[j]);
+                o += a.ldo;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; j++) {
+                if (j < lim) *o = Out<kType>::of(v[j]);
+                o += a.ldo;
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty0 + (uint32_t)(acc * 8));  // the leader issues the next MMA
+      }
+    }
+  } else {
+    // ---------------- scales: each warp fills its lane quarter with the same words
+    const int quarter = warp & 3;
+    const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
+    const uint32_t* rs = (const uint32_t*)a.row_scales;
+    const uint32_t* qs = (const uint32_t*)a.query_scales;
+    if (p0 < p1) {
+      Walk walk(a, p0);
+      int slot = 0;
+      uint32_t sphase = 0;
+      bool stop = false;
+      for (int64_t p = p0; p < p1 && !stop; p++) {
+        const Tile t = walk.at(p);
+        for (int w = 0; w * 4 < a.kchunks; w++) {
+          uint32_t r[4], q[8];
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int64_t row = t.row + (int)rank * 128 + c * 32 + lane;
+            r[c] = row < a.nrows ? __ldg(rs + row * a.scale_words + w) : 0u;
+          }
+#pragma unroll
+          for (int c = 0; c < 8; c++) {
+            const int64_t query = t.query + c * 32 + lane;
+            q[c] = c * 32 < t.width && query < a.nq ? __ldcg(qs + query * a.scale_words + w) : 0u;
+          }
+          bool ok = !*abort_flag && mbar_wait(&sempty[slot], sphase ^ 1u, a.timeout_ns, abort_flag);
+          if (!__all_sync(0xFFFFFFFFu, ok)) {
+            if (lane == 0) give_up();
+            stop = true;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t taddr =
+              tmem_base + ((uint32_t)(quarter * 32) << 16) + kScaleBase + (uint32_t)(slot * kSlotCols);
+          tmem_st_32x32b_x4(taddr, r);
+          tmem_st_32x32b_x8(taddr + 4, q);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(sfull0 + (uint32_t)(slot * 8));
+          if (++slot == kScaleSlots) {
+            slot = 0;
+            sphase ^= 1u;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync();  // the pair's MMAs, loads and epilogues are done with TMEM and shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+// Tiles before each group: one block, each thread a run of consecutive groups.
+__global__ void __launch_bounds__(1024) fp8_group_tiles_kernel(const int64_t* row_off, const int64_t* query_off,
+                                                               int64_t groups, int64_t nrows, int64_t nq,
+                                                               int64_t max_cols, int64_t* tile_off) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int64_t warp_sum[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t per = (groups + 1023) / 1024;
+  const int64_t g0 = tid * per, g1 = g0 + per < groups ? g0 + per : groups;
+  int64_t mine = 0;
+  for (int64_t g = g0; g < g1; g++) mine += group_of(row_off, query_off, g, nrows, nq, max_cols).tiles;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int64_t before = incl - mine;
+  for (int i = 0; i < warp; i++) before += warp_sum[i];
+  for (int64_t g = g0; g < g1; g++) {
+    tile_off[g] = before;
+    before += group_of(row_off, query_off, g, nrows, nq, max_cols).tiles;
+  }
+  if (g0 < groups && g1 == groups) tile_off[groups] = before;
+}
+
+template <int kType>
+cudaError_t launch_typed(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, size_t smem, bool after_prep,
+                         cudaStream_t st) {
+  auto kern = fp8_scores_kernel<kType>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * units));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_prep ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, maps, a);
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_group_tiles(const int64_t* row_off, const int64_t* query_off, int64_t groups, int64_t nrows,
+                                   int64_t nq, int64_t max_cols, int64_t* tile_off, cudaStream_t st) {
+  fp8_group_tiles_kernel<<<1, 1024, 0, st>>>(row_off, query_off, groups, nrows, nq, max_cols, tile_off);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& args, int out_type, int num_sms, bool after_prep,
+                              cudaStream_t st) {
+  Fp8ScoreArgs a = args;
+  const int64_t qt = (a.nq + kFp8MaxWidth - 1) / kFp8MaxWidth;
+  int64_t units = num_sms / 2;
+  if (a.row_off) {
+    a.width = (int)(a.nq < kFp8MaxWidth ? (a.nq + 31) / 32 * 32 : kFp8MaxWidth);  // widest possible tile
+  } else {
+    a.query_tiles = (int)qt;
+    a.width = (int)(((a.nq + qt - 1) / qt + 31) / 32 * 32);
+    a.tiles = (a.nrows + 255) / 256 * qt;
+    if (units > a.tiles) units = a.tiles;
+  }
+  if (units < 1) units = 1;
+  a.stages = (int)((kMaxSmem - 1024 - kBarrierBytes) / stage_bytes(a.width));
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  a.wait_first = after_prep;
+  const size_t smem = 1024 + a.stages * stage_bytes(a.width) + kBarrierBytes;
+  switch (out_type) {
+    case VX_F32: return launch_typed<VX_F32>(maps, a, (int)units, smem, after_prep, st);
+    case VX_F16: return launch_typed<VX_F16>(maps, a, (int)units, smem, after_prep, st);
+    case VX_BF16: return launch_typed<VX_BF16>(maps, a, (int)units, smem, after_prep, st);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace vx

@@ -17,6 +17,7 @@
 
 #include "../../include/vx.h"
 #include "common.cuh"
+#include "fp8.h"
 #include "gemm_scan.h"
 #include "internal.h"
 #include "ivfpq.h"
@@ -2538,6 +2539,287 @@ int vx_merge_shards_device(int32_t device, int32_t nshards, const int64_t* d_off
     VX_LAUNCH(1, launch_merge_shards(nshards, d_offsets, d_shard_ids, d_shard_scores, d_shard_counts,
                                      kin, nq, k, d_ids, d_scores, d_counts, (cudaStream_t)stream));
     return VX_OK;
+  });
+}
+
+// ------------------------------------------------------------------ 8-bit float rows
+namespace vx {
+namespace {
+
+// Makes `device` current for a call and puts the caller's device back afterwards.
+struct DeviceScope {
+  int before = -1;
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    if (before == device) before = -1;
+    else VX_CUDA(cudaSetDevice(device));
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+// What the calls need to know of a device, looked up once: the number of SMs, and a word that a
+// kernel whose wait ran out sets and the host reads without waiting (mapped host memory).
+struct Fp8Device {
+  int sms = 0;
+  volatile int32_t* err = nullptr;
+  int32_t* d_err = nullptr;
+};
+constexpr int kFp8Devices = 64;
+Fp8Device g_fp8_dev[kFp8Devices];
+std::mutex g_fp8_mu;
+
+int fp8_device(int device, Fp8Device** out) {
+  if (device < 0 || device >= kFp8Devices) return fail(VX_ERR_INVALID_ARGUMENT, "device %d out of range", device);
+  std::lock_guard<std::mutex> lock(g_fp8_mu);
+  Fp8Device& d = g_fp8_dev[device];
+  if (!d.err) {
+    int before = -1;
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    // a first call inside a stream capture allocates the word outside it
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const bool exchanged = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    int sms = 0;
+    const int status = check_device(device, &sms);
+    void *h = nullptr, *p = nullptr;
+    cudaError_t e = cudaSuccess;
+    if (status == VX_OK) {
+      e = cudaHostAlloc(&h, sizeof(int32_t), cudaHostAllocMapped | cudaHostAllocPortable);
+      if (e == cudaSuccess) e = cudaHostGetDevicePointer(&p, h, 0);
+    }
+    if (exchanged) cudaThreadExchangeStreamCaptureMode(&mode);
+    if (before >= 0) cudaSetDevice(before);
+    if (status != VX_OK) return status;
+    VX_CUDA(e);
+    *(int32_t*)h = 0;
+    d.sms = sms;
+    d.d_err = (int32_t*)p;
+    d.err = (volatile int32_t*)h;
+  }
+  *out = &d;
+  return VX_OK;
+}
+
+// A wait that ran out in an earlier call.
+int fp8_pending(Fp8Device* d) {
+  if (*d->err == 0) return VX_OK;
+  *d->err = 0;
+  return fail(VX_ERR_DEVICE_TIMEOUT, "a device-side wait of an 8-bit score product exceeded its time budget");
+}
+
+int elem_bytes_of(int type) { return type == VX_F32 ? 4 : type == VX_F16 || type == VX_BF16 ? 2 : 0; }
+bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
+
+int fp8_check_store(const void* codes, const void* scales, int64_t rows, int32_t dim) {
+  if (dim <= 0 || dim > kFp8MaxDim)
+    return fail(VX_ERR_INVALID_ARGUMENT, "dimension must be in [1, %d]: %d", kFp8MaxDim, dim);
+  if (rows < 0 || rows >= INT32_MAX)
+    return fail(VX_ERR_INVALID_ARGUMENT, "stored rows must be in [0, 2^31 - 1): %lld", (long long)rows);
+  if (rows > 0 && (!codes || !scales)) return fail(VX_ERR_NULL_POINTER, "codes and scales must not be null");
+  if (!aligned(codes, 16) || !aligned(scales, 4))
+    return fail(VX_ERR_INVALID_ARGUMENT, "codes must be 16-byte aligned and scales 4-byte aligned");
+  return VX_OK;
+}
+
+// A matrix of n rows of `width` elements, `stride` elements apart.
+int fp8_check_matrix(const char* what, const void* p, int type, int64_t n, int64_t width, int64_t stride) {
+  const int bytes = elem_bytes_of(type);
+  if (bytes == 0) return fail(VX_ERR_INVALID_ARGUMENT, "%s: unknown element type %d", what, type);
+  if (n > 0 && width > 0 && !p) return fail(VX_ERR_NULL_POINTER, "%s must not be null", what);
+  if (!aligned(p, (size_t)bytes)) return fail(VX_ERR_INVALID_ARGUMENT, "%s must be %d-byte aligned", what, bytes);
+  if (stride < width)
+    return fail(VX_ERR_INVALID_ARGUMENT, "%s: stride %lld below the row's %lld elements", what, (long long)stride,
+                (long long)width);
+  if (n > 0 && stride > INT64_MAX / 8 / n) return fail(VX_ERR_INVALID_ARGUMENT, "%s: too large", what);
+  return VX_OK;
+}
+
+int fp8_check_slots(const void* slots, int32_t slot_bytes, int64_t first, int64_t n, int64_t capacity) {
+  if (n < 0 || n >= INT32_MAX) return fail(VX_ERR_INVALID_ARGUMENT, "rows must be in [0, 2^31 - 1): %lld", (long long)n);
+  if (slots) {
+    if (slot_bytes != 4 && slot_bytes != 8)
+      return fail(VX_ERR_INVALID_ARGUMENT, "slots are 4- or 8-byte integers: %d", slot_bytes);
+    if (!aligned(slots, (size_t)slot_bytes)) return fail(VX_ERR_INVALID_ARGUMENT, "slots must be %d-byte aligned", slot_bytes);
+  } else if (first < 0 || first > capacity || n > capacity - first) {
+    return fail(VX_ERR_INVALID_ARGUMENT, "rows [%lld, %lld + %lld) do not fit a store of %lld", (long long)first,
+                (long long)first, (long long)n, (long long)capacity);
+  }
+  return VX_OK;
+}
+
+struct Fp8Queries {
+  const void* p;
+  int32_t type;
+  const uint8_t* scales;
+  int64_t nq, stride;
+};
+
+int fp8_check_queries(const Fp8Queries& q, int32_t dim) {
+  if (q.nq < 0 || q.nq >= INT32_MAX)
+    return fail(VX_ERR_INVALID_ARGUMENT, "queries must be in [0, 2^31 - 1): %lld", (long long)q.nq);
+  if (q.type == VX_E4M3) return fp8_check_store(q.p, q.scales, q.nq, dim);
+  return fp8_check_matrix("queries", q.p, q.type, q.nq, dim, q.stride);
+}
+
+// 2-D e4m3 operand [rows][pitch] with a (128-byte x box_rows) box.
+void fp8_map(CUtensorMap* m, const uint8_t* codes, int64_t rows, int pitch, int box_rows) {
+  make_tmap(m, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pitch, rows, box_rows);
+}
+
+// The queries quantised if they are floats, the groups' tiles counted, and the product.
+int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const uint8_t* scales, int64_t n, int32_t dim,
+               const int64_t* query_off, const int64_t* row_off, int64_t groups, void* out, int32_t out_type,
+               int64_t out_stride, int64_t max_cols, cudaStream_t st) {
+  Fp8Device* dev = nullptr;
+  if (int s = fp8_device(device, &dev)) return s;
+  if (int s = fp8_pending(dev)) return s;
+  if (n == 0 || q.nq == 0 || (row_off && (groups == 0 || max_cols == 0))) return VX_OK;
+  DeviceScope here(device);
+  Scratch S(st);
+  const int pitch = fp8_code_pitch(dim), scale_pitch = fp8_scale_pitch(dim);
+  const uint8_t *q_codes = (const uint8_t*)q.p, *q_scales = q.scales;
+  bool prep = false;
+  Fp8ScoreArgs a{};
+  if (row_off) {
+    int64_t* tile_off = S.alloc<int64_t>((size_t)groups + 1);
+    VX_LAUNCH(1, launch_fp8_group_tiles(row_off, query_off, groups, n, q.nq, max_cols, tile_off, st));
+    a.row_off = row_off;
+    a.query_off = query_off;
+    a.tile_off = tile_off;
+    a.groups = groups;
+    a.max_cols = max_cols;
+    prep = true;
+  }
+  if (q.type != VX_E4M3) {
+    uint8_t* buf = S.alloc<uint8_t>((size_t)q.nq * (pitch + scale_pitch));
+    q_codes = buf;
+    q_scales = buf + (size_t)q.nq * pitch;
+    Fp8WriteArgs w{};
+    w.rows = q.p;
+    w.type = q.type;
+    w.n = q.nq;
+    w.dim = dim;
+    w.stride = q.stride;
+    w.codes = buf;
+    w.scales = buf + (size_t)q.nq * pitch;
+    w.capacity = q.nq;
+    int launches = 0;
+    cudaError_t e = launch_fp8_write(w, true, &launches, st);
+    VX_LAUNCH(launches, e);
+    prep = true;
+  }
+  Fp8Maps maps;
+  fp8_map(&maps.rows, codes, n, pitch, 128);
+  for (int i = 0; i < 3; i++) fp8_map(&maps.queries[i], q_codes, q.nq, pitch, 64 >> i);
+  a.row_scales = scales;
+  a.nrows = n;
+  a.query_scales = q_scales;
+  a.nq = q.nq;
+  a.scale_words = scale_pitch / 4;
+  a.kchunks = pitch / 128;
+  a.out = out;
+  a.ldo = out_stride;
+  a.timeout_ns = wait_timeout_ns();
+  a.err = dev->d_err;
+  VX_LAUNCH(1, launch_fp8_scores(maps, a, out_type, dev->sms, prep, st));
+  return VX_OK;
+}
+
+}  // namespace
+}  // namespace vx
+
+int vx_fp8_pitch(int32_t dim, int32_t* code_pitch, int32_t* scale_pitch) {
+  return guarded([&]() -> int {
+    if (!code_pitch || !scale_pitch) return fail(VX_ERR_NULL_POINTER, "null output");
+    if (int s = fp8_check_store(nullptr, nullptr, 0, dim)) return s;
+    *code_pitch = fp8_code_pitch(dim);
+    *scale_pitch = fp8_scale_pitch(dim);
+    return VX_OK;
+  });
+}
+
+int vx_fp8_write_device(int32_t device, const void* rows, int32_t type, int64_t n, int32_t dim, int64_t row_stride,
+                        const void* slots, int32_t slot_bytes, int64_t first, uint8_t* codes, uint8_t* scales,
+                        int64_t capacity, void* stream) {
+  return guarded([&]() -> int {
+    if (int s = fp8_check_store(codes, scales, capacity, dim)) return s;
+    if (int s = fp8_check_slots(slots, slot_bytes, first, n, capacity)) return s;
+    if (int s = fp8_check_matrix("rows", rows, type, n, dim, row_stride)) return s;
+    Fp8Device* dev = nullptr;
+    if (int s = fp8_device(device, &dev)) return s;
+    if (n == 0 || capacity == 0) return VX_OK;
+    DeviceScope here(device);
+    cudaStream_t st = (cudaStream_t)stream;
+    Scratch S(st);
+    Fp8WriteArgs a{rows, type, n, dim, row_stride, slots, slot_bytes, first, codes, scales, capacity, nullptr};
+    if (slots && n > kFp8DirectSlots) a.owner = S.alloc<int32_t>((size_t)capacity);
+    int launches = 0;
+    cudaError_t e = launch_fp8_write(a, false, &launches, st);
+    VX_LAUNCH(launches, e);
+    return VX_OK;
+  });
+}
+
+int vx_fp8_read_device(int32_t device, const uint8_t* codes, const uint8_t* scales, int64_t capacity, int32_t dim,
+                       const void* slots, int32_t slot_bytes, int64_t first, int64_t n, void* out, int32_t out_type,
+                       int64_t out_stride, void* stream) {
+  return guarded([&]() -> int {
+    if (int s = fp8_check_store(codes, scales, capacity, dim)) return s;
+    if (int s = fp8_check_slots(slots, slot_bytes, first, n, capacity)) return s;
+    if (int s = fp8_check_matrix("out", out, out_type, n, dim, out_stride)) return s;
+    Fp8Device* dev = nullptr;
+    if (int s = fp8_device(device, &dev)) return s;
+    if (n == 0) return VX_OK;
+    DeviceScope here(device);
+    Fp8ReadArgs a{codes, scales, capacity, dim, slots, slot_bytes, first, n, out, out_type, out_stride};
+    VX_LAUNCH(1, launch_fp8_read(a, (cudaStream_t)stream));
+    return VX_OK;
+  });
+}
+
+int vx_fp8_scores_device(int32_t device, const void* queries, int32_t query_type, const uint8_t* query_scales, int64_t nq,
+                         int64_t query_stride, const uint8_t* codes, const uint8_t* scales, int64_t n, int32_t dim,
+                         void* out, int32_t out_type, int64_t out_stride, void* stream) {
+  return guarded([&]() -> int {
+    const Fp8Queries q{queries, query_type, query_scales, nq, query_stride};
+    if (nq == 0) return fail(VX_ERR_INVALID_ARGUMENT, "queries must not be empty");
+    if (int s = fp8_check_store(codes, scales, n, dim)) return s;
+    if (int s = fp8_check_queries(q, dim)) return s;
+    if (int s = fp8_check_matrix("out", out, out_type, nq, n, out_stride)) return s;
+    return fp8_scores(device, q, codes, scales, n, dim, nullptr, nullptr, 0, out, out_type, out_stride, n,
+                      (cudaStream_t)stream);
+  });
+}
+
+int vx_fp8_scores_grouped_device(int32_t device, const void* queries, int32_t query_type, const uint8_t* query_scales,
+                                 int64_t nq, int64_t query_stride, const int64_t* query_offsets, const uint8_t* codes,
+                                 const uint8_t* scales, int64_t n, const int64_t* row_offsets, int64_t groups,
+                                 int32_t dim, void* out, int32_t out_type, int64_t out_stride, int64_t max_rows,
+                                 void* stream) {
+  return guarded([&]() -> int {
+    const Fp8Queries q{queries, query_type, query_scales, nq, query_stride};
+    if (int s = fp8_check_store(codes, scales, n, dim)) return s;
+    if (int s = fp8_check_queries(q, dim)) return s;
+    if (groups < 0 || groups >= INT32_MAX)
+      return fail(VX_ERR_INVALID_ARGUMENT, "groups must be in [0, 2^31 - 1): %lld", (long long)groups);
+    if (groups > 0 && (!query_offsets || !row_offsets)) return fail(VX_ERR_NULL_POINTER, "offsets must not be null");
+    if (!aligned(query_offsets, 8) || !aligned(row_offsets, 8))
+      return fail(VX_ERR_INVALID_ARGUMENT, "offsets must be 8-byte aligned");
+    if (max_rows < 0) return fail(VX_ERR_INVALID_ARGUMENT, "max_rows must not be negative: %lld", (long long)max_rows);
+    if (int s = fp8_check_matrix("out", out, out_type, nq, max_rows, out_stride)) return s;
+    return fp8_scores(device, q, codes, scales, n, dim, query_offsets, row_offsets, groups, out, out_type, out_stride,
+                      max_rows, (cudaStream_t)stream);
+  });
+}
+
+int vx_fp8_check(int32_t device, void* stream) {
+  return guarded([&]() -> int {
+    Fp8Device* dev = nullptr;
+    if (int s = fp8_device(device, &dev)) return s;
+    DeviceScope here(device);
+    VX_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+    return fp8_pending(dev);
   });
 }
 
