@@ -76,11 +76,18 @@ struct Fp8ScoreArgs {
   int wait_first;
 };
 
-// The operands' tensor maps: `rows` with 128-row boxes, queries[i] with boxes of 64 >> i rows.
+// The operands' tensor maps: `rows` with 128-row boxes; queries[0] with boxes of half a tile's queries
+// (fp8_query_width), or with groups queries[i] with boxes of 64 >> i rows.
 struct Fp8Maps {
   CUtensorMap rows;
   CUtensorMap queries[3];
 };
+
+// Queries of one tile of an ungrouped product, in equal tiles of at most kFp8MaxWidth.
+inline int fp8_query_width(int64_t nq) {
+  const int64_t tiles = (nq + kFp8MaxWidth - 1) / kFp8MaxWidth;
+  return (int)(((nq + tiles - 1) / tiles + 31) / 32 * 32);
+}
 
 // Tiles before each group, from untrusted offsets (clamped to the operands' sizes).
 cudaError_t launch_fp8_group_tiles(const int64_t* row_off, const int64_t* query_off, int64_t groups, int64_t nrows,

@@ -17,13 +17,17 @@
 // chunk by TMA (128-byte swizzle).  224 and not 256 queries: two accumulators take 448 of the 512
 // TMEM columns and leave 60 for a ring of five scale slots.
 //
-// Scales.  A slot holds the scale words of four K chunks (512 dimensions): 4 columns for the CTA's
-// 128 rows and 8 for the queries.  A stored row's scale bytes are consecutive, so a 32-bit load
+// Scales.  A slot holds the scale words of four K chunks (512 dimensions): 128 words for the CTA's
+// rows and up to 256 for the queries.  A stored row's scale bytes are consecutive, so a 32-bit load
 // gives four chunks' exponents, which go to TMEM as they are (the descriptor's scale id picks the
-// byte).  Four warps per CTA, one for each TMEM lane quarter, load and store them.
+// byte).  Three warps copy them to shared memory (cp.async), a fourth hands a slot that has landed
+// to the MMA thread, which copies it to TMEM (tcgen05.cp) in the tensor core's own order ahead of
+// its MMAs.  (Stored from registers with tcgen05.st, or handed over by the loading warps, whose
+// release waits for their loads in flight, a slot took 1,400-2,000 cycles, more than its MMAs.)
 //
-// Warps: 0 TMA, 1 TMEM and (leader CTA) MMA, 2-5 epilogue, 6-9 scales.  Every wait is bounded; on
-// expiry the error word is set, the roles unwind and TMEM is released.
+// Warps: 0 rows by TMA, 1 TMEM and (leader CTA) MMA, 2-5 epilogue, 6 row scales, 7-8 query scales, 9
+// queries by TMA, 10 hand-over of scales.  Every wait is bounded; on expiry the error word is set, the roles unwind and
+// TMEM is released.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,14 +40,15 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;
 constexpr int kTmemCols = 512;
 constexpr int kRowBytes = 128 * 128;  // a CTA's stored-row operand per stage
 constexpr int kScaleSlots = 5;
 constexpr int kSlotCols = 12;
+constexpr int kSlotBytes = 1536;  // 128 row words, then up to 256 query words
 constexpr uint32_t kScaleBase = 2 * kFp8MaxWidth;
 constexpr size_t kMaxSmem = 232448;
-constexpr size_t kBarrierBytes = 512;
+constexpr size_t kTailBytes = kScaleSlots * kSlotBytes + 512;  // scale slots and barriers
 constexpr int kMaxStages = 12;
 
 static_assert(kScaleBase + kScaleSlots * kSlotCols <= kTmemCols, "TMEM columns");
@@ -79,43 +84,76 @@ __device__ __forceinline__ Group group_of(const int64_t* row_off, const int64_t*
   return r;
 }
 
-// Walks a work unit's tiles in order.  One group: tile t is (row tile t / query_tiles, query tile
-// t % query_tiles).  Several: the group of the unit's first tile by bisection of tile_off, later ones
-// by stepping.
+// The tiles of a work unit, in order, from number `p` of its range to before `end`.  One group: tile p
+// is (row tile p / query_tiles, query tile p % query_tiles), and the clusters take tiles in turn, so
+// that they work side by side (results of one query in neighbouring DRAM pages).  Several groups:
+// each cluster takes a run of consecutive tiles, so that stepping from group to group stays cheap.
 struct Walk {
   const Fp8ScoreArgs& a;
   Group g;
-  int64_t group;  // current group (groups only)
-  int64_t base;   // tiles before it
-  __device__ __forceinline__ Walk(const Fp8ScoreArgs& args, int64_t first) : a(args), group(0), base(0) {
+  int64_t p, end, step;
+  int64_t group;   // current group (groups only)
+  int64_t rt, qt;  // row and query tile within it
+  int64_t step_rt, step_qt;
+  __device__ __forceinline__ Walk(const Fp8ScoreArgs& args, int64_t unit, int64_t units) : a(args), group(0) {
     if (!a.row_off) {
       g.row0 = g.query0 = 0;
       g.nrows = a.nrows;
       g.nqueries = a.nq;
       g.query_tiles = a.query_tiles;
       g.width = a.width;
+      p = unit;
+      end = a.tiles;
+      step = units;
+      rt = p / a.query_tiles;
+      qt = p % a.query_tiles;
+      step_rt = units / a.query_tiles;
+      step_qt = units % a.query_tiles;
       return;
     }
-    int64_t lo = 0, hi = a.groups;  // tile_off[lo] <= first < tile_off[hi]
+    const int64_t total = a.tile_off[a.groups];
+    p = total * unit / units;
+    end = total * (unit + 1) / units;
+    step = step_qt = 1;
+    step_rt = rt = qt = 0;
+    if (p >= end) return;
+    int64_t lo = 0, hi = a.groups;  // tile_off[lo] <= p < tile_off[hi]; 32 places tried at once
     while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.tile_off[mid] <= first) lo = mid;
-      else hi = mid;
+      const int64_t by = (hi - lo + 31) >> 5;
+      const int64_t at = lo + by * ((threadIdx.x & 31) + 1);
+      const int k = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && a.tile_off[at] <= p));
+      lo += by * k;
+      if (lo + by < hi) hi = lo + by;
     }
     group = lo;
-    base = a.tile_off[lo];
     g = group_of(a.row_off, a.query_off, lo, a.nrows, a.nq, a.max_cols);
+    const int64_t t = p - a.tile_off[lo];
+    rt = t / (g.query_tiles > 0 ? g.query_tiles : 1);
+    qt = t - rt * g.query_tiles;
   }
-  __device__ __forceinline__ Tile at(int64_t p) {
-    if (a.row_off) {
-      while (p >= base + g.tiles && group + 1 < a.groups) {
-        base += g.tiles;
+  __device__ __forceinline__ bool more() const { return p < end; }
+  __device__ __forceinline__ int64_t count() const { return p < end ? (end - p + step - 1) / step : 0; }
+  __device__ __forceinline__ void next() {
+    p += step;
+    qt += step_qt;
+    rt += step_rt;
+    if (qt >= g.query_tiles) {
+      qt -= g.query_tiles;
+      rt++;
+    }
+    if (a.row_off && rt * 256 >= g.nrows && p < end) {  // on to the next group that has tiles
+      do {
+        if (group + 1 >= a.groups) {  // only if the offsets changed during the call
+          end = p;
+          return;
+        }
         group++;
         g = group_of(a.row_off, a.query_off, group, a.nrows, a.nq, a.max_cols);
-      }
+      } while (g.tiles == 0);
+      rt = qt = 0;
     }
-    const int64_t t = p - base;
-    const int64_t rt = t / g.query_tiles, qt = t % g.query_tiles;
+  }
+  __device__ __forceinline__ Tile tile() const {
     Tile x;
     x.row = g.row0 + rt * 256;
     x.col = a.row_off ? rt * 256 : x.row;
@@ -124,7 +162,8 @@ struct Walk {
     x.query = g.query0 + qt * g.width;
     const int64_t ql = g.nqueries - qt * g.width;
     x.queries = ql < g.width ? (int)(ql < 0 ? 0 : ql) : g.width;
-    x.width = x.queries > 0 ? (x.queries + 31) / 32 * 32 : 32;
+    // ungrouped tiles all load queries by boxes of half the width
+    x.width = !a.row_off ? a.width : x.queries > 0 ? (x.queries + 31) / 32 * 32 : 32;
     return x;
   }
 };
@@ -154,9 +193,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int n_stages = a.stages;
   const size_t stage_size = stage_bytes(a.width);
-  uint64_t* full = (uint64_t*)(stages + n_stages * stage_size);
+  uint8_t* slots = stages + n_stages * stage_size;
+  uint64_t* full = (uint64_t*)(slots + kScaleSlots * kSlotBytes);
   uint64_t* empty = full + kMaxStages;
-  uint64_t* sfull = empty + kMaxStages;
+  uint64_t* landed = empty + kMaxStages;
+  uint64_t* sfull = landed + kScaleSlots;
   uint64_t* sempty = sfull + kScaleSlots;
   uint64_t* tfull = sempty + kScaleSlots;
   uint64_t* tempty = tfull + 2;
@@ -164,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = (uint32_t*)(drained + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
@@ -175,7 +216,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kScaleSlots; s++) {
-      mbar_init(&sfull[s], 8);  // four scale warps of each CTA
+      mbar_init(&landed[s], 96);  // the lanes of the three loading warps
+      mbar_init(&sfull[s], 2);    // each CTA's hand-over
       mbar_init(&sempty[s], 1);
     }
     for (int b = 0; b < 2; b++) {
@@ -197,47 +239,52 @@ __global__ void __launch_bounds__(kThreads, 1)
   // The launch before this one wrote the encoded queries, the groups' tile counts or both.
   if (a.wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  const int64_t total = a.row_off ? a.tile_off[a.groups] : a.tiles;
-  const int64_t p0 = total * unit / units, p1 = total * (unit + 1) / units;
+  Walk walk(a, unit, units);
+  const bool any = walk.more();
 
   auto give_up = [&]() {
     *abort_flag = 1;
     record_error(a.err, kDevWaitTimeout);
   };
 
-  if (warp == 0) {
-    if (lane == 0 && p0 < p1) {
-      prefetch_tmap(&maps.rows);
-      for (int i = 0; i < 3; i++) prefetch_tmap(&maps.queries[i]);
-      const uint64_t pol_q = policy_evict_last();  // query tiles are read again for every row tile
-      const uint64_t pol_r = policy_evict_normal();
+  if (warp == 0 || warp == 9) {
+    // ---------------- TMA: warp 0 the stored rows, warp 9 the queries
+    if (any && elect_one()) {
+      const bool rows = warp == 0;
+      if (rows) prefetch_tmap(&maps.rows);
+      else prefetch_tmap(&maps.queries[0]);
+      // query tiles are read again for every row tile
+      const uint64_t policy = rows ? policy_evict_normal() : policy_evict_last();
       const uint32_t full0 = mapa_shared(smem_addr(&full[0]), 0);
       int stage = 0;
       uint32_t phase = 0;
-      Walk walk(a, p0);
-      for (int64_t p = p0; p < p1 && !*abort_flag; p++) {
-        const Tile t = walk.at(p);
+      for (; walk.more() && !*abort_flag; walk.next()) {
+        const Tile t = walk.tile();
         const int half = t.width >> 1;  // query rows of this CTA
-        const int32_t yr = (int32_t)t.row + (int)rank * 128;
-        const int32_t yq = (int32_t)t.query + (int)rank * half;
+        const int32_t y0 = rows ? (int32_t)t.row + (int)rank * 128 : (int32_t)t.query + (int)rank * half;
         for (int kc = 0; kc < a.kchunks; kc++) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, a.timeout_ns, abort_flag)) {
             give_up();
             break;
           }
           uint8_t* s = stages + stage * stage_size;
-          if (leader) mbar_arrive_expect_tx(&full[stage], 2u * (uint32_t)stage_bytes(t.width));
           const uint32_t bar = full0 + (uint32_t)(stage * 8);
-          tma_load_2d_pair(s, &maps.rows, bar, kc * 128, yr, pol_r);
-          s += kRowBytes;
-          int32_t y = yq;
+          if (rows) {
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2u * (uint32_t)stage_bytes(t.width));
+            tma_load_2d_pair(s, &maps.rows, bar, kc * 128, y0, policy);
+          } else if (!a.row_off) {
+            tma_load_2d_pair(s + kRowBytes, &maps.queries[0], bar, kc * 128, y0, policy);
+          } else {
+            int32_t y = y0;
+            s += kRowBytes;
 #pragma unroll
-          for (int i = 0; i < 3; i++) {  // the half's rows as boxes of 64, 32 and 16
-            const int box = 64 >> i;
-            if (half & box) {
-              tma_load_2d_pair(s, &maps.queries[i], bar, kc * 128, y, pol_q);
-              s += box * 128;
-              y += box;
+            for (int i = 0; i < 3; i++) {  // the half's rows as boxes of 64, 32 and 16
+              const int box = 64 >> i;
+              if (half & box) {
+                tma_load_2d_pair(s, &maps.queries[i], bar, kc * 128, y, policy);
+                s += box * 128;
+                y += box;
+              }
             }
           }
           if (++stage == n_stages) {
@@ -254,15 +301,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader && p0 < p1) {
+    if (leader && any && elect_one()) {
       int stage = 0, slot = 0;
       uint32_t phase = 0, sphase = 0;
-      Walk walk(a, p0);
-      for (int64_t p = p0; p < p1 && !*abort_flag; p++) {
-        const Tile t = walk.at(p);
-        const int64_t li = p - p0;
+      uint32_t li = 0;
+      for (; walk.more() && !*abort_flag; walk.next(), li++) {
+        const Tile t = walk.tile();
         const int acc = (int)(li & 1);
-        if (!mbar_wait(&tempty[acc], (uint32_t)((li >> 1) & 1) ^ 1u, a.timeout_ns, abort_flag)) {
+        if (!mbar_wait(&tempty[acc], ((li >> 1) & 1u) ^ 1u, a.timeout_ns, abort_flag)) {
           give_up();
           break;
         }
@@ -272,16 +318,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int kc = 0; kc < a.kchunks; kc++) {
           const int sub = kc & 3;
-          if (sub == 0 && !mbar_wait(&sfull[slot], sphase, a.timeout_ns, abort_flag)) ok = false;
-          if (ok && !mbar_wait(&full[stage], phase, a.timeout_ns, abort_flag)) ok = false;
-          if (!ok) {
+          const uint32_t scales = tmem_base + kScaleBase + (uint32_t)(slot * kSlotCols);
+          if (sub == 0) {
+            if (!mbar_wait(&sfull[slot], sphase, a.timeout_ns, abort_flag)) {
+              ok = false;
+              give_up();
+              break;
+            }
+            tc_fence_after();
+            const uint64_t ds = scale_block_desc(smem_addr(slots + slot * kSlotBytes));
+            tmem_cp_scales_pair(scales, ds);
+            tmem_cp_scales_pair(scales + 4, ds + (512 >> 4));
+            if (t.width > 128) tmem_cp_scales_pair(scales + 8, ds + (1024 >> 4));
+          }
+          if (!mbar_wait(&full[stage], phase, a.timeout_ns, abort_flag)) {
+            ok = false;
             give_up();
             break;
           }
           tc_fence_after();
           const uint32_t sa = smem_addr(stages + stage * stage_size);
           const uint64_t da = sw128_kmajor_desc(sa), db = sw128_kmajor_desc(sa + kRowBytes);
-          const uint32_t scales = tmem_base + kScaleBase + (uint32_t)(slot * kSlotCols);
           const uint32_t idesc = idesc0 | ((uint32_t)sub << 4) | ((uint32_t)sub << 29);
 #pragma unroll
           for (int kk = 0; kk < 4; kk++)
@@ -315,95 +372,103 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;
     const int my_row = (int)rank * 128 + quarter * 32 + lane;
     const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0);
-    if (p0 < p1) {
-      Walk walk(a, p0);
-      for (int64_t p = p0; p < p1; p++) {
-        const Tile t = walk.at(p);
-        const int64_t li = p - p0;
-        const int acc = (int)(li & 1);
-        const bool row_in = my_row < t.rows;
-        T* out = (T*)a.out + t.query * a.ldo + t.col + my_row;
-        if (__shfl_sync(0xFFFFFFFFu, *abort_flag, 0)) break;
-        const bool ok = mbar_wait(&tfull[acc], (uint32_t)((li >> 1) & 1), a.timeout_ns, abort_flag);
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
-          if (lane == 0) give_up();
-          break;
-        }
-        tc_fence_after();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * kFp8MaxWidth);
-        for (int c0 = 0; c0 < t.queries; c0 += 32) {
-          uint32_t v[32];
-          __syncwarp();
-          tmem_ld_32x32b_x32(taddr + (uint32_t)c0, v);
-          tmem_ld_wait_v(v);
-          const int lim = t.queries - c0;
-          if (row_in) {
-            T* o = out + c0 * a.ldo;
-            if (lim >= 32) {
+    uint32_t li = 0;
+    for (; walk.more(); walk.next(), li++) {
+      const Tile t = walk.tile();
+      const int acc = (int)(li & 1);
+      const bool row_in = my_row < t.rows;
+      T* out = (T*)a.out + t.query * a.ldo + t.col + my_row;
+      if (__shfl_sync(0xFFFFFFFFu, *abort_flag, 0)) break;
+      const bool ok = mbar_wait(&tfull[acc], (li >> 1) & 1u, a.timeout_ns, abort_flag);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        if (lane == 0) give_up();
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * kFp8MaxWidth);
+      for (int c0 = 0; c0 < t.queries; c0 += 32) {
+        uint32_t v[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(taddr + (uint32_t)c0, v);
+        tmem_ld_wait_v(v);
+        const int lim = t.queries - c0;
+        if (row_in) {
+          T* o = out + c0 * a.ldo;
+          if (lim >= 32) {
 #pragma unroll
-              for (int j = 0; j < 32; j++) {
-                *o = Out<kType>::of(v[j]);
-                o += a.ldo;
-              }
-            } else {
+            for (int j = 0; j < 32; j++) {
+              *o = Out<kType>::of(v[j]);
+              o += a.ldo;
+            }
+          } else {
 #pragma unroll
-              for (int j = 0; j < 32; j++) {
-                if (j < lim) *o = Out<kType>::of(v[j]);
-                o += a.ldo;
-              }
+            for (int j = 0; j < 32; j++) {
+              if (j < lim) *o = Out<kType>::of(v[j]);
+              o += a.ldo;
             }
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tempty0 + (uint32_t)(acc * 8));  // the leader issues the next MMA
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + (uint32_t)(acc * 8));  // the leader issues the next MMA
     }
-  } else {
-    // ---------------- scales: each warp fills its lane quarter with the same words
-    const int quarter = warp & 3;
-    const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
-    const uint32_t* rs = (const uint32_t*)a.row_scales;
-    const uint32_t* qs = (const uint32_t*)a.query_scales;
-    if (p0 < p1) {
-      Walk walk(a, p0);
-      int slot = 0;
-      uint32_t sphase = 0;
-      bool stop = false;
-      for (int64_t p = p0; p < p1 && !stop; p++) {
-        const Tile t = walk.at(p);
-        for (int w = 0; w * 4 < a.kchunks; w++) {
-          uint32_t r[4], q[8];
+  } else if (warp < 9) {
+    // ---------------- scales: warp 6 the CTA's 128 rows, warps 7 and 8 the tile's queries 0-127 and
+    // 128-223, lane l the words of rows l, 32 + l, 64 + l and 96 + l (the order TMEM has them in)
+    const int part = warp - 6;
+    const uint8_t* src = part == 0 ? a.row_scales : a.query_scales;
+    const int64_t limit = part == 0 ? a.nrows : a.nq;
+    const int slots_per_tile = (a.kchunks + 3) >> 2;
+    int slot = 0;
+    uint32_t sphase = 0;
+    for (; walk.more(); walk.next()) {
+      const Tile t = walk.tile();
+      const int64_t first = (part == 0 ? t.row + (int)rank * 128 : t.query + (part - 1) * 128) + lane;
+      const int count = part == 0 ? 128 : t.width - (part - 1) * 128;
+      const uint8_t* at[4];
+      bool in[4];
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const int64_t row = t.row + (int)rank * 128 + c * 32 + lane;
-            r[c] = row < a.nrows ? __ldg(rs + row * a.scale_words + w) : 0u;
-          }
-#pragma unroll
-          for (int c = 0; c < 8; c++) {
-            const int64_t query = t.query + c * 32 + lane;
-            q[c] = c * 32 < t.width && query < a.nq ? __ldcg(qs + query * a.scale_words + w) : 0u;
-          }
-          bool ok = !*abort_flag && mbar_wait(&sempty[slot], sphase ^ 1u, a.timeout_ns, abort_flag);
-          if (!__all_sync(0xFFFFFFFFu, ok)) {
-            if (lane == 0) give_up();
-            stop = true;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t taddr =
-              tmem_base + ((uint32_t)(quarter * 32) << 16) + kScaleBase + (uint32_t)(slot * kSlotCols);
-          tmem_st_32x32b_x4(taddr, r);
-          tmem_st_32x32b_x8(taddr + 4, q);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(sfull0 + (uint32_t)(slot * 8));
-          if (++slot == kScaleSlots) {
-            slot = 0;
-            sphase ^= 1u;
-          }
+      for (int c = 0; c < 4; c++) {
+        const int64_t row = first + c * 32;
+        in[c] = c * 32 < count && row < limit;
+        at[c] = in[c] ? src + row * (4 * (int64_t)a.scale_words) : src;
+      }
+      bool ok = true;
+      for (int w = 0; w < slots_per_tile; w++) {
+        ok = !*abort_flag && mbar_wait(&sempty[slot], sphase ^ 1u, a.timeout_ns, abort_flag);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) {
+          if (lane == 0) give_up();
+          break;
         }
+        const uint32_t dst = smem_addr(slots + slot * kSlotBytes + part * 512 + lane * 16);
+#pragma unroll
+        for (int c = 0; c < 4; c++) cp_async_4(dst + 4 * c, at[c] + 4 * w, in[c]);
+        cp_async_arrive(&landed[slot]);
+        if (++slot == kScaleSlots) {
+          slot = 0;
+          sphase ^= 1u;
+        }
+      }
+      if (!ok) break;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (any && elect_one()) {
+    // ---------------- warp 10: slots that have landed go to the leader's MMA thread
+    const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
+    int slot = 0;
+    uint32_t sphase = 0;
+    for (int64_t left = walk.count() * ((a.kchunks + 3) >> 2); left > 0; left--) {
+      if (*abort_flag || !mbar_wait(&landed[slot], sphase, a.timeout_ns, abort_flag)) {
+        give_up();
+        break;
+      }
+      fence_proxy_async();
+      mbar_arrive_cluster(sfull0 + (uint32_t)(slot * 8));
+      if (++slot == kScaleSlots) {
+        slot = 0;
+        sphase ^= 1u;
       }
     }
   }
@@ -484,15 +549,15 @@ cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& args, int
     a.width = (int)(a.nq < kFp8MaxWidth ? (a.nq + 31) / 32 * 32 : kFp8MaxWidth);  // widest possible tile
   } else {
     a.query_tiles = (int)qt;
-    a.width = (int)(((a.nq + qt - 1) / qt + 31) / 32 * 32);
+    a.width = fp8_query_width(a.nq);
     a.tiles = (a.nrows + 255) / 256 * qt;
     if (units > a.tiles) units = a.tiles;
   }
   if (units < 1) units = 1;
-  a.stages = (int)((kMaxSmem - 1024 - kBarrierBytes) / stage_bytes(a.width));
+  a.stages = (int)((kMaxSmem - 1024 - kTailBytes) / stage_bytes(a.width));
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   a.wait_first = after_prep;
-  const size_t smem = 1024 + a.stages * stage_bytes(a.width) + kBarrierBytes;
+  const size_t smem = 1024 + a.stages * stage_bytes(a.width) + kTailBytes;
   switch (out_type) {
     case VX_F32: return launch_typed<VX_F32>(maps, a, (int)units, smem, after_prep, st);
     case VX_F16: return launch_typed<VX_F16>(maps, a, (int)units, smem, after_prep, st);

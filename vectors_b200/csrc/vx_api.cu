@@ -2709,9 +2709,12 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
     VX_LAUNCH(launches, e);
     prep = true;
   }
-  Fp8Maps maps;
+  Fp8Maps maps{};
   fp8_map(&maps.rows, codes, n, pitch, 128);
-  for (int i = 0; i < 3; i++) fp8_map(&maps.queries[i], q_codes, q.nq, pitch, 64 >> i);
+  if (!row_off)
+    fp8_map(&maps.queries[0], q_codes, q.nq, pitch, fp8_query_width(q.nq) / 2);
+  else
+    for (int i = 0; i < 3; i++) fp8_map(&maps.queries[i], q_codes, q.nq, pitch, 64 >> i);
   a.row_scales = scales;
   a.nrows = n;
   a.query_scales = q_scales;
