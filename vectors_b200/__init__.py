@@ -5,15 +5,6 @@ list scan) run as hand-written CUDA kernels in ``libvx.so``; this package is the
 mirror of the reference's index SPI over that library's C ABI (include/vx.h).
 """
 from ._native import VxError, device_count, kernel_launches, lib  # noqa: F401
-from .fp8 import (  # noqa: F401
-    fp8_check,
-    fp8_empty,
-    fp8_pitch,
-    fp8_read_device,
-    fp8_scores_device,
-    fp8_scores_grouped_device,
-    fp8_write_device,
-)
 from .index_spi import (  # noqa: F401
     FlatScanAdapter,
     GpuUnavailableException,
@@ -62,3 +53,15 @@ __all__ = [
     "lib",
     "VxError",
 ]
+
+_FP8 = frozenset(n for n in __all__ if n.startswith("fp8_"))
+
+
+def __getattr__(name):
+    """The 8-bit row functions (fp8.py) work on torch tensors; torch is imported with the first of them."""
+    if name in _FP8:
+        from . import fp8
+
+        globals().update({n: getattr(fp8, n) for n in _FP8})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

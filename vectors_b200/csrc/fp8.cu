@@ -8,9 +8,9 @@
 // byte, and the tensor cores apply it inside the product (fp8_scores.cu).  A block that holds a
 // NaN or an infinity is NaN throughout: scale byte 255, codes 0x7f.
 //
-// Both kernels stream: per row they move dim elements and pitch(dim) codes + scales, and one warp
-// takes four blocks (512 dimensions) of one row, 4 elements a lane and block, so that the four
-// blocks' loads are in flight together and their scales make one 32-bit word.
+// Both kernels stream: per row they move dim elements and pitch(dim) codes + scales.  One warp takes
+// up to kWords x 4 blocks of one row, 4 elements a lane and block: their loads are in flight
+// together, every access of the warp is consecutive, and four blocks' scales make one 32-bit word.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -21,6 +21,7 @@
 #include "../../include/vx.h"
 #include "common.cuh"
 #include "fp8.h"
+#include "fp8_groups.cuh"
 
 namespace vx {
 namespace {
@@ -88,92 +89,119 @@ __device__ __forceinline__ int scale_byte(uint32_t amax_bits) {
 // Where several rows of a batch name one slot, the last of them is kept.  Up to kFp8DirectSlots
 // rows: each row looks for its slot among the later rows.  Above: owner[slot] becomes the largest
 // row index that names the slot, without clearing `owner` first: every row stores its index (some
-// row's index is left), then every row raises the entry to its own.
-__global__ void owner_store_kernel(const void* slots, int slot_bytes, int64_t n, int64_t capacity, int32_t* owner) {
+// row's index is left), then every row raises the entry to its own.  The three launches overlap:
+// each begins before the one before it ends and waits for it where it needs its results.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <bool kMax>
+__global__ void owner_kernel(const void* slots, int slot_bytes, int64_t n, int64_t capacity, int32_t* owner) {
+  launch_dependents();
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int64_t s = slot_at(slots, slot_bytes, i);
-  if (s >= 0 && s < capacity) owner[s] = (int32_t)i;
-}
-__global__ void owner_max_kernel(const void* slots, int slot_bytes, int64_t n, int64_t capacity, int32_t* owner) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int64_t s = slot_at(slots, slot_bytes, i);
-  if (s >= 0 && s < capacity) atomicMax(&owner[s], (int32_t)i);
+  const int64_t s = i < n ? slot_at(slots, slot_bytes, i) : -1;
+  if (kMax) wait_for_launch_before();
+  if (s < 0 || s >= capacity) return;
+  if (kMax) atomicMax(&owner[s], (int32_t)i);
+  else owner[s] = (int32_t)i;
 }
 
 // ---------------------------------------------------------------- write
-template <class T, bool kVec>
-__global__ void __launch_bounds__(kThreads) fp8_write_kernel(const Fp8WriteArgs a, int words, bool early) {
-  if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+// Blocks of 8 warps; block b takes rows 8 (b / parts) + warp, part b % parts of their words.
+// kGroups: block 0 counts a grouped product's tiles instead.
+template <class T, bool kVec, int kWords, bool kGroups>
+__global__ void __launch_bounds__(kThreads) fp8_write_kernel(const Fp8WriteArgs a, const Fp8Groups groups, uint32_t parts) {
+  launch_dependents();
+  uint32_t block = blockIdx.x;
+  if constexpr (kGroups) {
+    if (block == 0) {
+      fp8_count_tiles<kThreads>(groups);
+      return;
+    }
+    block--;
+  }
   const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t row = unit / words;
-  const int w = (int)(unit % words);  // blocks 4w .. 4w + 3
-  if (row >= a.n) return;
-  int64_t slot = a.first + row;
+  const int64_t row = (int64_t)(block / parts) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int first = (int)(block % parts) * kWords * 4;  // first block of the row's
+  const int nb = (a.dim + kFp8Block - 1) / kFp8Block;
+  const T* x = (const T*)a.rows + row * a.stride;
+  float v[kWords * 4][4];
+  int64_t slot = -1;
+  if (row < a.n) {
+#pragma unroll
+    for (int j = 0; j < kWords * 4; j++) load4<T, kVec>(x, (first + j) * kFp8Block + lane * 4, a.dim, v[j]);
+    slot = a.slots ? slot_at(a.slots, a.slot_bytes, row) : a.first + row;
+  }
+  if (a.owner) wait_for_launch_before();  // every thread: no block ends before the launches before it
+  if (slot < 0 || slot >= a.capacity) return;
   if (a.slots) {
-    slot = slot_at(a.slots, a.slot_bytes, row);
-    if (slot < 0 || slot >= a.capacity) return;
     if (a.owner) {
-      if (a.owner[slot] != (int32_t)row) return;
+      if (__ldcg(a.owner + slot) != (int32_t)row) return;
     } else {
       bool later = false;
       for (int64_t j = row + 1 + lane; j < a.n; j += 32) later |= slot_at(a.slots, a.slot_bytes, j) == slot;
       if (__any_sync(0xFFFFFFFFu, later)) return;
     }
   }
-  const int nb = (a.dim + kFp8Block - 1) / kFp8Block;
-  const T* x = (const T*)a.rows + row * a.stride;
-  float v[4][4];
-#pragma unroll
-  for (int j = 0; j < 4; j++) load4<T, kVec>(x, (4 * w + j) * kFp8Block + lane * 4, a.dim, v[j]);
-  uint32_t word = 0;
   uint8_t* codes = a.codes + slot * ((int64_t)nb * kFp8Block);
+  uint8_t* scales = a.scales + slot * (int64_t)((nb + 3) / 4 * 4);
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    uint32_t m = 0;
+  for (int w = 0; w < kWords; w++) {
+    if (first + 4 * w >= nb) break;
+    uint32_t word = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
-    m = __reduce_max_sync(0xFFFFFFFFu, m);
-    if (4 * w + j >= nb) break;
-    const int b = scale_byte(m);
-    word |= (uint32_t)b << (8 * j);
-    uint32_t c = 0x7F7F7F7Fu;
-    if (b != 255) {
-      const float inv = __uint_as_float((uint32_t)(254 - b) << 23);  // 2^(127 - b), b <= 247
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[j][0] * inv, v[j][1] * inv), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[j][2] * inv, v[j][3] * inv), __NV_SATFINITE, __NV_E4M3);
-      c = lo | (hi << 16);
+    for (int j = 0; j < 4; j++) {
+      const float(&y)[4] = v[4 * w + j];
+      const int k = first + 4 * w + j;
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+      m = __reduce_max_sync(0xFFFFFFFFu, m);
+      if (k >= nb) break;
+      const int b = scale_byte(m);
+      word |= (uint32_t)b << (8 * j);
+      uint32_t c = 0x7F7F7F7Fu;
+      if (b != 255) {
+        const float inv = __uint_as_float((uint32_t)(254 - b) << 23);  // 2^(127 - b), b <= 247
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0] * inv, y[1] * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2] * inv, y[3] * inv), __NV_SATFINITE, __NV_E4M3);
+        c = lo | (hi << 16);
+      }
+      *(uint32_t*)(codes + k * kFp8Block + lane * 4) = c;
     }
-    *(uint32_t*)(codes + (4 * w + j) * kFp8Block + lane * 4) = c;
+    if (lane == 0) *(uint32_t*)(scales + first + 4 * w) = word;
   }
-  if (lane == 0) *(uint32_t*)(a.scales + slot * (4 * (int64_t)words) + 4 * w) = word;
+}
+
+__global__ void __launch_bounds__(1024) fp8_count_tiles_kernel(const Fp8Groups groups) {
+  launch_dependents();
+  fp8_count_tiles<1024>(groups);
 }
 
 // ---------------------------------------------------------------- read
-template <class T, bool kVec>
-__global__ void __launch_bounds__(kThreads) fp8_read_kernel(const Fp8ReadArgs a, int words) {
+template <class T, bool kVec, int kWords>
+__global__ void __launch_bounds__(kThreads) fp8_read_kernel(const Fp8ReadArgs a, uint32_t parts) {
   const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t row = unit / words;
-  const int w = (int)(unit % words);
+  const int64_t row = (int64_t)(blockIdx.x / parts) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int first = (int)(blockIdx.x % parts) * kWords * 4;
   if (row >= a.n) return;
   const int64_t slot = a.slots ? slot_at(a.slots, a.slot_bytes, row) : a.first + row;
   const bool in = slot >= 0 && slot < a.capacity;
   const int nb = (a.dim + kFp8Block - 1) / kFp8Block;
   const uint8_t* codes = a.codes + (in ? slot : 0) * ((int64_t)nb * kFp8Block);
-  uint32_t c[4], word = 0;
-  if (in) word = __ldg((const uint32_t*)(a.scales + slot * (4 * (int64_t)words) + 4 * w));
+  const uint8_t* scales = a.scales + (in ? slot : 0) * (int64_t)((nb + 3) / 4 * 4);
+  uint32_t c[kWords * 4], word[kWords];
 #pragma unroll
-  for (int j = 0; j < 4; j++)
-    c[j] = in && 4 * w + j < nb ? __ldcs((const uint32_t*)(codes + (4 * w + j) * kFp8Block + lane * 4)) : 0u;
+  for (int w = 0; w < kWords; w++)
+    word[w] = in && first + 4 * w < nb ? __ldg((const uint32_t*)(scales + first + 4 * w)) : 0u;
+#pragma unroll
+  for (int j = 0; j < kWords * 4; j++)
+    c[j] = in && first + j < nb ? __ldcs((const uint32_t*)(codes + (first + j) * kFp8Block + lane * 4)) : 0u;
   T* y = (T*)a.out + row * a.stride;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int k = (4 * w + j) * kFp8Block + lane * 4;
+  for (int j = 0; j < kWords * 4; j++) {
+    const int k = (first + j) * kFp8Block + lane * 4;
     if (k >= a.dim) break;
-    const uint32_t b = (word >> (8 * j)) & 0xFFu;
+    const uint32_t b = (word[j >> 2] >> (8 * (j & 3))) & 0xFFu;
     // 2^(b - 127); b = 0 is the subnormal 2^-127, 255 is NaN
     const float s = __uint_as_float(b == 255u ? 0x7FC00000u : b == 0u ? 0x00400000u : b << 23);
     const __half2 lo = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c[j] & 0xFFFFu), __NV_E4M3));
@@ -199,53 +227,98 @@ bool four_aligned(const void* p, int64_t stride) {
   return (uintptr_t)p % (4 * sizeof(T)) == 0 && stride % 4 == 0;
 }
 
-template <class T>
-cudaError_t write_typed(const Fp8WriteArgs& a, bool early, int words, unsigned grid, cudaStream_t st) {
+// Parts of a row of `words` scale words that a warp each takes, and the blocks for n rows.
+int parts_of(int words, int per) { return (words + per - 1) / per; }
+bool grid_for(int64_t n, int parts, int extra, unsigned* grid) {
+  const int64_t g = (n + kThreads / 32 - 1) / (kThreads / 32) * parts + extra;
+  *grid = (unsigned)g;
+  return g <= 0x7FFFFFFF;
+}
+
+// Launches `kern`, allowed to begin before the launch before it ends if `dependent`.
+template <class... P, class... A>
+cudaError_t launch(void (*kern)(P...), unsigned grid, int threads, bool dependent, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <class T, int kWords, bool kGroups>
+cudaError_t write_words(const Fp8WriteArgs& a, const Fp8Groups& g, int words, cudaStream_t st) {
+  const int parts = parts_of(words, kWords);
+  unsigned grid;
+  if (!grid_for(a.n, parts, kGroups ? 1 : 0, &grid)) return cudaErrorInvalidValue;
+  const bool dependent = a.owner != nullptr;
   if (four_aligned<T>(a.rows, a.stride))
-    fp8_write_kernel<T, true><<<grid, kThreads, 0, st>>>(a, words, early);
-  else
-    fp8_write_kernel<T, false><<<grid, kThreads, 0, st>>>(a, words, early);
-  return cudaGetLastError();
+    return launch(fp8_write_kernel<T, true, kWords, kGroups>, grid, kThreads, dependent, st, a, g, (uint32_t)parts);
+  return launch(fp8_write_kernel<T, false, kWords, kGroups>, grid, kThreads, dependent, st, a, g, (uint32_t)parts);
 }
 
-template <class T>
-cudaError_t read_typed(const Fp8ReadArgs& a, int words, unsigned grid, cudaStream_t st) {
-  if (four_aligned<T>(a.out, a.stride))
-    fp8_read_kernel<T, true><<<grid, kThreads, 0, st>>>(a, words);
-  else
-    fp8_read_kernel<T, false><<<grid, kThreads, 0, st>>>(a, words);
-  return cudaGetLastError();
-}
-
-}  // namespace
-
-cudaError_t launch_fp8_write(const Fp8WriteArgs& a, bool early, int* launches, cudaStream_t st) {
+// Rows of more than 512 dimensions: a warp takes 8 blocks (kWords 2), else 4.
+template <class T, bool kGroups>
+cudaError_t write_typed(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st) {
   const int words = fp8_scale_pitch(a.dim) / 4;
-  *launches = 1;
-  if (a.owner) {
-    const unsigned g = (unsigned)((a.n + kThreads - 1) / kThreads);
-    owner_store_kernel<<<g, kThreads, 0, st>>>(a.slots, a.slot_bytes, a.n, a.capacity, a.owner);
-    owner_max_kernel<<<g, kThreads, 0, st>>>(a.slots, a.slot_bytes, a.n, a.capacity, a.owner);
-    *launches = 3;
-  }
-  const int64_t grid = (a.n * words + kThreads / 32 - 1) / (kThreads / 32);
-  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  return words > 1 ? write_words<T, 2, kGroups>(a, g, words, st) : write_words<T, 1, kGroups>(a, g, words, st);
+}
+
+template <bool kGroups>
+cudaError_t write_any(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st) {
   switch (a.type) {
-    case VX_F32: return write_typed<float>(a, early, words, (unsigned)grid, st);
-    case VX_F16: return write_typed<__half>(a, early, words, (unsigned)grid, st);
-    case VX_BF16: return write_typed<__nv_bfloat16>(a, early, words, (unsigned)grid, st);
+    case VX_F32: return write_typed<float, kGroups>(a, g, st);
+    case VX_F16: return write_typed<__half, kGroups>(a, g, st);
+    case VX_BF16: return write_typed<__nv_bfloat16, kGroups>(a, g, st);
     default: return cudaErrorInvalidValue;
   }
 }
 
-cudaError_t launch_fp8_read(const Fp8ReadArgs& a, cudaStream_t st) {
+template <class T, int kWords>
+cudaError_t read_words(const Fp8ReadArgs& a, int words, cudaStream_t st) {
+  const int parts = parts_of(words, kWords);
+  unsigned grid;
+  if (!grid_for(a.n, parts, 0, &grid)) return cudaErrorInvalidValue;
+  if (four_aligned<T>(a.out, a.stride))
+    return launch(fp8_read_kernel<T, true, kWords>, grid, kThreads, false, st, a, (uint32_t)parts);
+  return launch(fp8_read_kernel<T, false, kWords>, grid, kThreads, false, st, a, (uint32_t)parts);
+}
+
+template <class T>
+cudaError_t read_typed(const Fp8ReadArgs& a, cudaStream_t st) {
   const int words = fp8_scale_pitch(a.dim) / 4;
-  const int64_t grid = (a.n * words + kThreads / 32 - 1) / (kThreads / 32);
-  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  return words > 1 ? read_words<T, 2>(a, words, st) : read_words<T, 1>(a, words, st);
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_write(const Fp8WriteArgs& a, int* launches, cudaStream_t st) {
+  *launches = 1;
+  if (a.owner) {
+    const unsigned g = (unsigned)((a.n + kThreads - 1) / kThreads);
+    cudaError_t e = launch(owner_kernel<false>, g, kThreads, false, st, a.slots, a.slot_bytes, a.n, a.capacity, a.owner);
+    if (e == cudaSuccess)
+      e = launch(owner_kernel<true>, g, kThreads, true, st, a.slots, a.slot_bytes, a.n, a.capacity, a.owner);
+    if (e != cudaSuccess) return e;
+    *launches = 3;
+  }
+  return write_any<false>(a, Fp8Groups{}, st);
+}
+
+cudaError_t launch_fp8_prepare(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st) {
+  if (!a.rows) return launch(fp8_count_tiles_kernel, 1u, 1024, false, st, g);
+  return g.row_off ? write_any<true>(a, g, st) : write_any<false>(a, g, st);
+}
+
+cudaError_t launch_fp8_read(const Fp8ReadArgs& a, cudaStream_t st) {
   switch (a.type) {
-    case VX_F32: return read_typed<float>(a, words, (unsigned)grid, st);
-    case VX_F16: return read_typed<__half>(a, words, (unsigned)grid, st);
-    case VX_BF16: return read_typed<__nv_bfloat16>(a, words, (unsigned)grid, st);
+    case VX_F32: return read_typed<float>(a, st);
+    case VX_F16: return read_typed<__half>(a, st);
+    case VX_BF16: return read_typed<__nv_bfloat16>(a, st);
     default: return cudaErrorInvalidValue;
   }
 }

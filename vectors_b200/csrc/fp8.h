@@ -19,6 +19,16 @@ inline int fp8_blocks(int dim) { return (dim + kFp8Block - 1) / kFp8Block; }
 inline int fp8_code_pitch(int dim) { return fp8_blocks(dim) * kFp8Block; }  // bytes of codes per row
 inline int fp8_scale_pitch(int dim) { return (fp8_blocks(dim) + 3) / 4 * 4; }  // bytes of scales per row
 
+// A grouped product's offsets, the sizes they are clamped to, and where the tiles before each group go.
+struct Fp8Groups {
+  const int64_t* row_off;    // [groups + 1]; null: one group of every row and query
+  const int64_t* query_off;  // [groups + 1]
+  int64_t groups;
+  int64_t nrows, nq;
+  int64_t max_cols;   // results kept per query (groups with more rows are cut there)
+  int64_t* tile_off;  // [groups + 1]
+};
+
 struct Fp8WriteArgs {
   const void* rows;  // [n] rows, `stride` elements apart
   int type;          // vx_dtype of the rows
@@ -47,8 +57,10 @@ struct Fp8ReadArgs {
   int64_t stride;
 };
 
-// `early`: the kernel lets a dependent launch begin before it ends.
-cudaError_t launch_fp8_write(const Fp8WriteArgs& a, bool early, int* launches, cudaStream_t st);
+cudaError_t launch_fp8_write(const Fp8WriteArgs& a, int* launches, cudaStream_t st);
+// Before a product: quantises its queries (a.rows null: they are stored rows already) and counts the
+// groups' tiles (g.row_off null: no groups), in one launch that lets a dependent one begin early.
+cudaError_t launch_fp8_prepare(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st);
 cudaError_t launch_fp8_read(const Fp8ReadArgs& a, cudaStream_t st);
 
 struct Fp8ScoreArgs {
@@ -60,12 +72,7 @@ struct Fp8ScoreArgs {
   int kchunks;      // 128-byte chunks of a row
   void* out;
   int64_t ldo;  // elements between two queries' results
-  // one group of every row and query: row_off null
-  const int64_t* row_off;    // [groups + 1]
-  const int64_t* query_off;  // [groups + 1]
-  const int64_t* tile_off;   // [groups + 1], from launch_fp8_group_tiles
-  int64_t groups;
-  int64_t max_cols;  // results kept per query (groups with more rows are cut there)
+  Fp8Groups groups;
   uint64_t timeout_ns;
   int32_t* err;
   // filled in by launch_fp8_scores
@@ -89,11 +96,8 @@ inline int fp8_query_width(int64_t nq) {
   return (int)(((nq + tiles - 1) / tiles + 31) / 32 * 32);
 }
 
-// Tiles before each group, from untrusted offsets (clamped to the operands' sizes).
-cudaError_t launch_fp8_group_tiles(const int64_t* row_off, const int64_t* query_off, int64_t groups, int64_t nrows,
-                                   int64_t nq, int64_t max_cols, int64_t* tile_off, cudaStream_t st);
-// after_prep: the launch before this one on `st` is a kernel of this file's that encoded the
-// queries or counted the groups' tiles; this launch may begin before that one ends.
+// after_prep: the launch before this one on `st` is launch_fp8_prepare's; this one may begin before it
+// ends.
 cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& a, int out_type, int num_sms, bool after_prep,
                               cudaStream_t st);
 

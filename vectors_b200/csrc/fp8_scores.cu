@@ -31,8 +31,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "../../include/vx.h"
 #include "fp8.h"
+#include "fp8_groups.cuh"
 #include "sm100.cuh"
 
 namespace vx {
@@ -63,40 +66,19 @@ struct Tile {
   int width;    // MMA N: queries rounded up to 32
 };
 
-__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t hi) { return v < 0 ? 0 : v > hi ? hi : v; }
-
-// A group's rows and queries from its (untrusted) offsets.
-struct Group {
-  int64_t row0, nrows, query0, nqueries;
-  int64_t query_tiles, tiles;
-  int width;
-};
-__device__ __forceinline__ Group group_of(const int64_t* row_off, const int64_t* query_off, int64_t g, int64_t nrows,
-                                          int64_t nq, int64_t max_cols) {
-  Group r;
-  r.row0 = clamp64(row_off[g], nrows);
-  r.nrows = clamp64(clamp64(row_off[g + 1], nrows) - r.row0, max_cols);
-  r.query0 = clamp64(query_off[g], nq);
-  r.nqueries = clamp64(clamp64(query_off[g + 1], nq) - r.query0, nq);
-  r.query_tiles = (r.nqueries + kFp8MaxWidth - 1) / kFp8MaxWidth;
-  r.width = r.query_tiles ? (int)(((r.nqueries + r.query_tiles - 1) / r.query_tiles + 31) / 32 * 32) : 32;
-  r.tiles = (r.nrows + 255) / 256 * r.query_tiles;
-  return r;
-}
-
 // The tiles of a work unit, in order, from number `p` of its range to before `end`.  One group: tile p
 // is (row tile p / query_tiles, query tile p % query_tiles), and the clusters take tiles in turn, so
 // that they work side by side (results of one query in neighbouring DRAM pages).  Several groups:
 // each cluster takes a run of consecutive tiles, so that stepping from group to group stays cheap.
 struct Walk {
   const Fp8ScoreArgs& a;
-  Group g;
+  Fp8Group g;
   int64_t p, end, step;
   int64_t group;   // current group (groups only)
   int64_t rt, qt;  // row and query tile within it
   int64_t step_rt, step_qt;
   __device__ __forceinline__ Walk(const Fp8ScoreArgs& args, int64_t unit, int64_t units) : a(args), group(0) {
-    if (!a.row_off) {
+    if (!a.groups.row_off) {
       g.row0 = g.query0 = 0;
       g.nrows = a.nrows;
       g.nqueries = a.nq;
@@ -111,23 +93,23 @@ struct Walk {
       step_qt = units % a.query_tiles;
       return;
     }
-    const int64_t total = a.tile_off[a.groups];
+    const int64_t total = a.groups.tile_off[a.groups.groups];
     p = total * unit / units;
     end = total * (unit + 1) / units;
     step = step_qt = 1;
     step_rt = rt = qt = 0;
     if (p >= end) return;
-    int64_t lo = 0, hi = a.groups;  // tile_off[lo] <= p < tile_off[hi]; 32 places tried at once
+    int64_t lo = 0, hi = a.groups.groups;  // tile_off[lo] <= p < tile_off[hi]; 32 places tried at once
     while (hi - lo > 1) {
       const int64_t by = (hi - lo + 31) >> 5;
       const int64_t at = lo + by * ((threadIdx.x & 31) + 1);
-      const int k = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && a.tile_off[at] <= p));
+      const int k = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && a.groups.tile_off[at] <= p));
       lo += by * k;
       if (lo + by < hi) hi = lo + by;
     }
     group = lo;
-    g = group_of(a.row_off, a.query_off, lo, a.nrows, a.nq, a.max_cols);
-    const int64_t t = p - a.tile_off[lo];
+    g = fp8_group(a.groups, lo);
+    const int64_t t = p - a.groups.tile_off[lo];
     rt = t / (g.query_tiles > 0 ? g.query_tiles : 1);
     qt = t - rt * g.query_tiles;
   }
@@ -141,14 +123,14 @@ struct Walk {
       qt -= g.query_tiles;
       rt++;
     }
-    if (a.row_off && rt * 256 >= g.nrows && p < end) {  // on to the next group that has tiles
+    if (a.groups.row_off && rt * 256 >= g.nrows && p < end) {  // on to the next group that has tiles
       do {
-        if (group + 1 >= a.groups) {  // only if the offsets changed during the call
+        if (group + 1 >= a.groups.groups) {  // only if the offsets changed during the call
           end = p;
           return;
         }
         group++;
-        g = group_of(a.row_off, a.query_off, group, a.nrows, a.nq, a.max_cols);
+        g = fp8_group(a.groups, group);
       } while (g.tiles == 0);
       rt = qt = 0;
     }
@@ -156,14 +138,14 @@ struct Walk {
   __device__ __forceinline__ Tile tile() const {
     Tile x;
     x.row = g.row0 + rt * 256;
-    x.col = a.row_off ? rt * 256 : x.row;
+    x.col = a.groups.row_off ? rt * 256 : x.row;
     const int64_t rl = g.nrows - rt * 256;
     x.rows = rl < 256 ? (int)rl : 256;
     x.query = g.query0 + qt * g.width;
     const int64_t ql = g.nqueries - qt * g.width;
     x.queries = ql < g.width ? (int)(ql < 0 ? 0 : ql) : g.width;
     // ungrouped tiles all load queries by boxes of half the width
-    x.width = !a.row_off ? a.width : x.queries > 0 ? (x.queries + 31) / 32 * 32 : 32;
+    x.width = !a.groups.row_off ? a.width : x.queries > 0 ? (x.queries + 31) / 32 * 32 : 32;
     return x;
   }
 };
@@ -272,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rows) {
             if (leader) mbar_arrive_expect_tx(&full[stage], 2u * (uint32_t)stage_bytes(t.width));
             tma_load_2d_pair(s, &maps.rows, bar, kc * 128, y0, policy);
-          } else if (!a.row_off) {
+          } else if (!a.groups.row_off) {
             tma_load_2d_pair(s + kRowBytes, &maps.queries[0], bar, kc * 128, y0, policy);
           } else {
             int32_t y = y0;
@@ -481,40 +463,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Tiles before each group: one block, each thread a run of consecutive groups.
-__global__ void __launch_bounds__(1024) fp8_group_tiles_kernel(const int64_t* row_off, const int64_t* query_off,
-                                                               int64_t groups, int64_t nrows, int64_t nq,
-                                                               int64_t max_cols, int64_t* tile_off) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ int64_t warp_sum[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t per = (groups + 1023) / 1024;
-  const int64_t g0 = tid * per, g1 = g0 + per < groups ? g0 + per : groups;
-  int64_t mine = 0;
-  for (int64_t g = g0; g < g1; g++) mine += group_of(row_off, query_off, g, nrows, nq, max_cols).tiles;
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  int64_t before = incl - mine;
-  for (int i = 0; i < warp; i++) before += warp_sum[i];
-  for (int64_t g = g0; g < g1; g++) {
-    tile_off[g] = before;
-    before += group_of(row_off, query_off, g, nrows, nq, max_cols).tiles;
-  }
-  if (g0 < groups && g1 == groups) tile_off[groups] = before;
-}
-
 template <int kType>
 cudaError_t launch_typed(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, size_t smem, bool after_prep,
                          cudaStream_t st) {
   auto kern = fp8_scores_kernel<kType>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+  static std::atomic<uint64_t> sized{0};  // bit d: done for device d
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
+  if (device >= 64 || !((sized.load() >> device) & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+    if (e != cudaSuccess) return e;
+    if (device < 64) sized.fetch_or(1ull << device);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * units));
   cfg.blockDim = dim3(kThreads);
@@ -534,18 +495,12 @@ cudaError_t launch_typed(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, 
 
 }  // namespace
 
-cudaError_t launch_fp8_group_tiles(const int64_t* row_off, const int64_t* query_off, int64_t groups, int64_t nrows,
-                                   int64_t nq, int64_t max_cols, int64_t* tile_off, cudaStream_t st) {
-  fp8_group_tiles_kernel<<<1, 1024, 0, st>>>(row_off, query_off, groups, nrows, nq, max_cols, tile_off);
-  return cudaGetLastError();
-}
-
 cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& args, int out_type, int num_sms, bool after_prep,
                               cudaStream_t st) {
   Fp8ScoreArgs a = args;
   const int64_t qt = (a.nq + kFp8MaxWidth - 1) / kFp8MaxWidth;
   int64_t units = num_sms / 2;
-  if (a.row_off) {
+  if (a.groups.row_off) {
     a.width = (int)(a.nq < kFp8MaxWidth ? (a.nq + 31) / 32 * 32 : kFp8MaxWidth);  // widest possible tile
   } else {
     a.query_tiles = (int)qt;

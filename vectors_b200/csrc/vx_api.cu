@@ -2679,35 +2679,26 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
   Scratch S(st);
   const int pitch = fp8_code_pitch(dim), scale_pitch = fp8_scale_pitch(dim);
   const uint8_t *q_codes = (const uint8_t*)q.p, *q_scales = q.scales;
-  bool prep = false;
+  const bool encode = q.type != VX_E4M3;
+  const size_t q_bytes = encode ? (size_t)q.nq * (pitch + scale_pitch) : 0;
+  const size_t off_bytes = row_off ? ((size_t)groups + 1) * sizeof(int64_t) : 0;
   Fp8ScoreArgs a{};
-  if (row_off) {
-    int64_t* tile_off = S.alloc<int64_t>((size_t)groups + 1);
-    VX_LAUNCH(1, launch_fp8_group_tiles(row_off, query_off, groups, n, q.nq, max_cols, tile_off, st));
-    a.row_off = row_off;
-    a.query_off = query_off;
-    a.tile_off = tile_off;
-    a.groups = groups;
-    a.max_cols = max_cols;
-    prep = true;
-  }
-  if (q.type != VX_E4M3) {
-    uint8_t* buf = S.alloc<uint8_t>((size_t)q.nq * (pitch + scale_pitch));
-    q_codes = buf;
-    q_scales = buf + (size_t)q.nq * pitch;
-    Fp8WriteArgs w{};
-    w.rows = q.p;
-    w.type = q.type;
-    w.n = q.nq;
-    w.dim = dim;
-    w.stride = q.stride;
-    w.codes = buf;
-    w.scales = buf + (size_t)q.nq * pitch;
-    w.capacity = q.nq;
-    int launches = 0;
-    cudaError_t e = launch_fp8_write(w, true, &launches, st);
-    VX_LAUNCH(launches, e);
-    prep = true;
+  Fp8WriteArgs w{};
+  if (encode || row_off) {
+    uint8_t* buf = S.alloc<uint8_t>(round_up(off_bytes, 128) + q_bytes);
+    if (row_off) a.groups = Fp8Groups{row_off, query_off, groups, n, q.nq, max_cols, (int64_t*)buf};
+    if (encode) {
+      w.rows = q.p;
+      w.type = q.type;
+      w.n = w.capacity = q.nq;
+      w.dim = dim;
+      w.stride = q.stride;
+      w.codes = buf + round_up(off_bytes, 128);
+      w.scales = w.codes + (size_t)q.nq * pitch;
+      q_codes = w.codes;
+      q_scales = w.scales;
+    }
+    VX_LAUNCH(1, launch_fp8_prepare(w, a.groups, st));
   }
   Fp8Maps maps{};
   fp8_map(&maps.rows, codes, n, pitch, 128);
@@ -2725,7 +2716,7 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
   a.ldo = out_stride;
   a.timeout_ns = wait_timeout_ns();
   a.err = dev->d_err;
-  VX_LAUNCH(1, launch_fp8_scores(maps, a, out_type, dev->sms, prep, st));
+  VX_LAUNCH(1, launch_fp8_scores(maps, a, out_type, dev->sms, encode || row_off, st));
   return VX_OK;
 }
 
@@ -2758,7 +2749,7 @@ int vx_fp8_write_device(int32_t device, const void* rows, int32_t type, int64_t 
     Fp8WriteArgs a{rows, type, n, dim, row_stride, slots, slot_bytes, first, codes, scales, capacity, nullptr};
     if (slots && n > kFp8DirectSlots) a.owner = S.alloc<int32_t>((size_t)capacity);
     int launches = 0;
-    cudaError_t e = launch_fp8_write(a, false, &launches, st);
+    cudaError_t e = launch_fp8_write(a, &launches, st);
     VX_LAUNCH(launches, e);
     return VX_OK;
   });
