@@ -22,8 +22,8 @@
 // gives four chunks' exponents, which go to TMEM as they are (the descriptor's scale id picks the
 // byte).  Three warps copy them to shared memory (cp.async), a fourth hands a slot that has landed
 // to the MMA thread, which copies it to TMEM (tcgen05.cp) in the tensor core's own order ahead of
-// its MMAs.  (Stored from registers with tcgen05.st, or handed over by the loading warps, whose
-// release waits for their loads in flight, a slot took 1,400-2,000 cycles, more than its MMAs.)
+// its MMAs.  (Stored from registers with tcgen05.st, or handed over with a release at cluster scope,
+// a slot took 1,400-2,000 cycles, more than its MMAs.)
 //
 // Warps: 0 rows by TMA, 1 TMEM and (leader CTA) MMA, 2-5 epilogue, 6 row scales, 7-8 query scales, 9
 // queries by TMA, 10 hand-over of scales.  Every wait is bounded; on expiry the error word is set, the roles unwind and
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       fence_proxy_async();
-      mbar_arrive_cluster(sfull0 + (uint32_t)(slot * 8));
+      mbar_arrive_pair(sfull0 + (uint32_t)(slot * 8));
       if (++slot == kScaleSlots) {
         slot = 0;
         sphase ^= 1u;

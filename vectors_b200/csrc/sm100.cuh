@@ -220,10 +220,15 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // The same without ordering this thread's memory accesses before it: for hand-overs that carry no
-// data (TMEM that has been read).  The release above waits for the thread's outstanding global
-// loads and stores.
+// data (TMEM that has been read).  The release at cluster scope above waits for the SM's memory
+// traffic: about 2,000 cycles under load.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same with the default release (CTA scope): for shared memory of this CTA that its own barriers
+// have shown to be written, and that the pair's tensor cores read once the arrival is seen.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // 4-byte copy from global to shared memory (zero when !valid), and an arrival on `bar` when all of
 // this thread's copies so far have landed.
