@@ -25,8 +25,9 @@
 // its MMAs.  (Stored from registers with tcgen05.st, or handed over with a release at cluster scope,
 // a slot took 1,400-2,000 cycles, more than its MMAs.)
 //
-// Warps: 0 rows by TMA, 1 TMEM and (leader CTA) MMA, 2-5 epilogue, 6 row scales, 7-8 query scales, 9
-// queries by TMA, 10 hand-over of scales.  Every wait is bounded; on expiry the error word is set, the roles unwind and
+// Warps: 0 rows by TMA, 1 TMEM and (leader CTA) MMA, 2 row scales, 3-4 query scales, 5 hand-over of
+// scales, 6 queries by TMA, 8-15 epilogue (two per TMEM lane quarter, taking 32-query groups in
+// turn).  Every wait is bounded; on expiry the error word is set, the roles unwind and
 // TMEM is released.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,7 +44,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kThreads = 352;
+constexpr int kThreads = 512;
 constexpr int kTmemCols = 512;
 constexpr int kRowBytes = 128 * 128;  // a CTA's stored-row operand per stage
 constexpr int kScaleSlots = 5;
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 8);  // four epilogue warps of each CTA
+      mbar_init(&tempty[b], 16);  // eight epilogue warps of each CTA
     }
     mbar_init(drained, 1);
     *abort_flag = 0;
@@ -229,8 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     record_error(a.err, kDevWaitTimeout);
   };
 
-  if (warp == 0 || warp == 9) {
-    // ---------------- TMA: warp 0 the stored rows, warp 9 the queries
+  if (warp == 0 || warp == 6) {
+    // ---------------- TMA: warp 0 the stored rows, warp 6 the queries
     if (any && elect_one()) {
       const bool rows = warp == 0;
       if (rows) prefetch_tmap(&maps.rows);
@@ -348,10 +349,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (warp < 6) {
+  } else if (warp >= 8) {
     // ---------------- epilogue: one stored row per lane, one query per TMEM column
     using T = typename Out<kType>::T;
     const int quarter = warp & 3;
+    const int first = (warp >> 2 & 1) * 32;  // this warp's 32-query groups: every other one
     const int my_row = (int)rank * 128 + quarter * 32 + lane;
     const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0);
     uint32_t li = 0;
@@ -359,23 +361,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tile t = walk.tile();
       const int acc = (int)(li & 1);
       const bool row_in = my_row < t.rows;
-      T* out = (T*)a.out + t.query * a.ldo + t.col + my_row;
-      if (__shfl_sync(0xFFFFFFFFu, *abort_flag, 0)) break;
-      const bool ok = mbar_wait(&tfull[acc], (li >> 1) & 1u, a.timeout_ns, abort_flag);
+      T* o = (T*)a.out + (t.query + first) * a.ldo + t.col + my_row;
+      const bool ok = !*abort_flag && mbar_wait(&tfull[acc], (li >> 1) & 1u, a.timeout_ns, abort_flag);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         if (lane == 0) give_up();
         break;
       }
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * kFp8MaxWidth);
-      for (int c0 = 0; c0 < t.queries; c0 += 32) {
+      for (int c0 = first; c0 < t.queries; c0 += 64) {
         uint32_t v[32];
         __syncwarp();
         tmem_ld_32x32b_x32(taddr + (uint32_t)c0, v);
         tmem_ld_wait_v(v);
         const int lim = t.queries - c0;
         if (row_in) {
-          T* o = out + c0 * a.ldo;
           if (lim >= 32) {
 #pragma unroll
             for (int j = 0; j < 32; j++) {
@@ -389,16 +389,17 @@ __global__ void __launch_bounds__(kThreads, 1)
               o += a.ldo;
             }
           }
+          o += 32 * a.ldo;
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + (uint32_t)(acc * 8));  // the leader issues the next MMA
     }
-  } else if (warp < 9) {
-    // ---------------- scales: warp 6 the CTA's 128 rows, warps 7 and 8 the tile's queries 0-127 and
+  } else if (warp < 5) {
+    // ---------------- scales: warp 2 the CTA's 128 rows, warps 3 and 4 the tile's queries 0-127 and
     // 128-223, lane l the words of rows l, 32 + l, 64 + l and 96 + l (the order TMEM has them in)
-    const int part = warp - 6;
+    const int part = warp - 2;
     const uint8_t* src = part == 0 ? a.row_scales : a.query_scales;
     const int64_t limit = part == 0 ? a.nrows : a.nq;
     const int slots_per_tile = (a.kchunks + 3) >> 2;
@@ -436,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (any && elect_one()) {
-    // ---------------- warp 10: slots that have landed go to the leader's MMA thread
+  } else if (warp == 5 && any && elect_one()) {
+    // ---------------- slots that have landed go to the leader's MMA thread
     const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
     int slot = 0;
     uint32_t sphase = 0;
