@@ -109,8 +109,10 @@ __global__ void owner_kernel(const void* slots, int slot_bytes, int64_t n, int64
 // Blocks of 8 warps; block b takes rows 8 (b / parts) + warp, part b % parts of their words.
 // kGroups: block 0 counts a grouped product's tiles instead.
 template <class T, bool kVec, int kWords, bool kGroups>
-__global__ void __launch_bounds__(kThreads) fp8_write_kernel(const Fp8WriteArgs a, const Fp8Groups groups, uint32_t parts) {
+__global__ void __launch_bounds__(kThreads) fp8_write_kernel(const Fp8WriteArgs a, const Fp8Groups groups,
+                                                             unsigned long long* counter, uint32_t parts) {
   launch_dependents();
+  if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;
   uint32_t block = blockIdx.x;
   if constexpr (kGroups) {
     if (block == 0) {
@@ -172,8 +174,10 @@ __global__ void __launch_bounds__(kThreads) fp8_write_kernel(const Fp8WriteArgs 
   }
 }
 
-__global__ void __launch_bounds__(1024) fp8_count_tiles_kernel(const Fp8Groups groups) {
+__global__ void __launch_bounds__(1024) fp8_count_tiles_kernel(const Fp8Groups groups, unsigned long long* counter) {
   launch_dependents();
+  if (counter && threadIdx.x == 0) *counter = 0;
+  if (!groups.row_off) return;
   fp8_count_tiles<1024>(groups);
 }
 
@@ -251,29 +255,30 @@ cudaError_t launch(void (*kern)(P...), unsigned grid, int threads, bool dependen
 }
 
 template <class T, int kWords, bool kGroups>
-cudaError_t write_words(const Fp8WriteArgs& a, const Fp8Groups& g, int words, cudaStream_t st) {
+cudaError_t write_words(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, int words, cudaStream_t st) {
   const int parts = parts_of(words, kWords);
   unsigned grid;
   if (!grid_for(a.n, parts, kGroups ? 1 : 0, &grid)) return cudaErrorInvalidValue;
   const bool dependent = a.owner != nullptr;
   if (four_aligned<T>(a.rows, a.stride))
-    return launch(fp8_write_kernel<T, true, kWords, kGroups>, grid, kThreads, dependent, st, a, g, (uint32_t)parts);
-  return launch(fp8_write_kernel<T, false, kWords, kGroups>, grid, kThreads, dependent, st, a, g, (uint32_t)parts);
+    return launch(fp8_write_kernel<T, true, kWords, kGroups>, grid, kThreads, dependent, st, a, g, counter, (uint32_t)parts);
+  return launch(fp8_write_kernel<T, false, kWords, kGroups>, grid, kThreads, dependent, st, a, g, counter, (uint32_t)parts);
 }
 
 // Rows of more than 512 dimensions: a warp takes 8 blocks (kWords 2), else 4.
 template <class T, bool kGroups>
-cudaError_t write_typed(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st) {
+cudaError_t write_typed(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, cudaStream_t st) {
   const int words = fp8_scale_pitch(a.dim) / 4;
-  return words > 1 ? write_words<T, 2, kGroups>(a, g, words, st) : write_words<T, 1, kGroups>(a, g, words, st);
+  return words > 1 ? write_words<T, 2, kGroups>(a, g, counter, words, st)
+                   : write_words<T, 1, kGroups>(a, g, counter, words, st);
 }
 
 template <bool kGroups>
-cudaError_t write_any(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st) {
+cudaError_t write_any(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, cudaStream_t st) {
   switch (a.type) {
-    case VX_F32: return write_typed<float, kGroups>(a, g, st);
-    case VX_F16: return write_typed<__half, kGroups>(a, g, st);
-    case VX_BF16: return write_typed<__nv_bfloat16, kGroups>(a, g, st);
+    case VX_F32: return write_typed<float, kGroups>(a, g, counter, st);
+    case VX_F16: return write_typed<__half, kGroups>(a, g, counter, st);
+    case VX_BF16: return write_typed<__nv_bfloat16, kGroups>(a, g, counter, st);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -306,12 +311,12 @@ cudaError_t launch_fp8_write(const Fp8WriteArgs& a, int* launches, cudaStream_t 
     if (e != cudaSuccess) return e;
     *launches = 3;
   }
-  return write_any<false>(a, Fp8Groups{}, st);
+  return write_any<false>(a, Fp8Groups{}, nullptr, st);
 }
 
-cudaError_t launch_fp8_prepare(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st) {
-  if (!a.rows) return launch(fp8_count_tiles_kernel, 1u, 1024, false, st, g);
-  return g.row_off ? write_any<true>(a, g, st) : write_any<false>(a, g, st);
+cudaError_t launch_fp8_prepare(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, cudaStream_t st) {
+  if (!a.rows) return launch(fp8_count_tiles_kernel, 1u, 1024, false, st, g, counter);
+  return g.row_off ? write_any<true>(a, g, counter, st) : write_any<false>(a, g, counter, st);
 }
 
 cudaError_t launch_fp8_read(const Fp8ReadArgs& a, cudaStream_t st) {

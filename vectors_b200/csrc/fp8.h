@@ -26,6 +26,7 @@ struct Fp8Groups {
   int64_t groups;
   int64_t nrows, nq;
   int64_t max_cols;   // results kept per query (groups with more rows are cut there)
+  int tile_rows;      // stored rows of a tile
   int64_t* tile_off;  // [groups + 1]
 };
 
@@ -59,8 +60,9 @@ struct Fp8ReadArgs {
 
 cudaError_t launch_fp8_write(const Fp8WriteArgs& a, int* launches, cudaStream_t st);
 // Before a product: quantises its queries (a.rows null: they are stored rows already) and counts the
-// groups' tiles (g.row_off null: no groups), in one launch that lets a dependent one begin early.
-cudaError_t launch_fp8_prepare(const Fp8WriteArgs& a, const Fp8Groups& g, cudaStream_t st);
+// groups' tiles (g.row_off null: no groups), in one launch that lets a dependent one begin early; clears
+// *counter, unless null.
+cudaError_t launch_fp8_prepare(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, cudaStream_t st);
 cudaError_t launch_fp8_read(const Fp8ReadArgs& a, cudaStream_t st);
 
 struct Fp8ScoreArgs {
@@ -75,27 +77,30 @@ struct Fp8ScoreArgs {
   Fp8Groups groups;
   uint64_t timeout_ns;
   int32_t* err;
+  unsigned long long* next_tile;  // zero at the launch: tiles are taken from here; null: in fixed turns
+  int64_t tiles;      // without groups
+  int query_tiles;    // without groups
+  int width;          // queries of the widest tile, a multiple of 32
+  int tile_rows;      // stored rows of a tile
   // filled in by launch_fp8_scores
-  int64_t tiles;
-  int query_tiles;
-  int width;
   int stages;
+  int tile_slots;
   int wait_first;
 };
 
-// The operands' tensor maps: `rows` with 128-row boxes; queries[0] with boxes of half a tile's queries
-// (fp8_query_width), or with groups queries[i] with boxes of 64 >> i rows.
+// The operands' tensor maps: `rows` with boxes of half a tile's rows; queries[0] with boxes of half a
+// tile's queries, or with groups queries[i] with boxes of 64 >> i rows.
 struct Fp8Maps {
   CUtensorMap rows;
   CUtensorMap queries[3];
 };
 
-// Queries of one tile of an ungrouped product, in equal tiles of at most kFp8MaxWidth.
-inline int fp8_query_width(int64_t nq) {
-  const int64_t tiles = (nq + kFp8MaxWidth - 1) / kFp8MaxWidth;
-  return (int)(((nq + tiles - 1) / tiles + 31) / 32 * 32);
-}
-
+// The tiling of a product: tile sizes and, without groups, the number of tiles.
+struct Fp8Tiling {
+  int width, tile_rows, query_tiles;
+  int64_t tiles;
+};
+Fp8Tiling fp8_tiling(int64_t nrows, int64_t nq, int64_t groups, int num_sms);
 // after_prep: the launch before this one on `st` is launch_fp8_prepare's; this one may begin before it
 // ends.
 cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& a, int out_type, int num_sms, bool after_prep,

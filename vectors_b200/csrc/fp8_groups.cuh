@@ -19,11 +19,11 @@ __device__ __forceinline__ Fp8Group fp8_group(const Fp8Groups& a, int64_t g) {
   r.nrows = clamp_to(clamp_to(a.row_off[g + 1], a.nrows) - r.row0, a.max_cols);
   r.query0 = clamp_to(a.query_off[g], a.nq);
   r.nqueries = clamp_to(clamp_to(a.query_off[g + 1], a.nq) - r.query0, a.nq);
-  r.query_tiles = (r.nqueries + kFp8MaxWidth - 1) / kFp8MaxWidth;
-  // up to 2^31 queries and 2^23 tiles of them: 32-bit division
+  // rows and queries are below 2^31: 32-bit division
+  r.query_tiles = (uint32_t)(r.nqueries + kFp8MaxWidth - 1) / (uint32_t)kFp8MaxWidth;
   r.width = r.query_tiles == 0 ? 32
                                : (int)(((uint32_t)(r.nqueries + r.query_tiles - 1) / (uint32_t)r.query_tiles + 31) / 32 * 32);
-  r.tiles = (r.nrows + 255) / 256 * r.query_tiles;
+  r.tiles = (int64_t)((uint32_t)(r.nrows + a.tile_rows - 1) / (uint32_t)a.tile_rows) * r.query_tiles;
   return r;
 }
 

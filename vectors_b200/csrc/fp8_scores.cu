@@ -10,8 +10,11 @@
 // MMAs themselves.)
 //
 // Tiling.  2-CTA clusters (cta_group::2), 256 stored rows x up to 224 queries.  The stored rows are
-// the MMA's M operand, so a TMEM lane holds one stored row and an epilogue warp writes 32
-// consecutive results of one query at a time: coalesced, with no transposition.  The queries are
+// the MMA's M operand, so a TMEM lane holds one stored row and an epilogue warp has 32 consecutive
+// results of each query, which it stores as they are: 32 lanes, 4 (or 2) bytes each.  (16 bytes a
+// lane, brought together by shuffles or through shared memory, or TMA stores from there, were
+// slower: 400 MB of fp32 results 115, 90 and 89 us against 85; 200 MB of bf16 84, 68 and 91 against
+// 50.)  The queries are
 // its N operand, any multiple of 32, so few queries cost few MMA cycles and the kernel then streams
 // the stored rows at HBM speed; each CTA stages its 128 rows and half the queries of a 128-byte K
 // chunk by TMA (128-byte swizzle).  224 and not 256 queries: two accumulators take 448 of the 512
@@ -25,8 +28,13 @@
 // its MMAs.  (Stored from registers with tcgen05.st, or handed over with a release at cluster scope,
 // a slot took 1,400-2,000 cycles, more than its MMAs.)
 //
+// Tiles.  Clusters take tiles from a counter, not in fixed turns: with large results the SMs' shares
+// of the write bandwidth differ by half (the slowest unit of 1000 x 100k fp32 results took 87 us
+// with the median at 67).  One warp of the leader finds the next tile, with groups by a search over
+// 32 places at once, and sends its description to every role of both CTAs.
+//
 // Warps: 0 rows by TMA, 1 TMEM and (leader CTA) MMA, 2 row scales, 3-4 query scales, 5 hand-over of
-// scales, 6 queries by TMA, 8-15 epilogue (two per TMEM lane quarter, taking 32-query groups in
+// scales, 6 queries by TMA, 7 (leader CTA) tiles, 8-15 epilogue (two per TMEM lane quarter, taking 32-query groups in
 // turn).  Every wait is bounded; on expiry the error word is set, the roles unwind and
 // TMEM is released.
 #include <cuda_bf16.h>
@@ -52,101 +60,88 @@ constexpr int kSlotCols = 12;
 constexpr int kSlotBytes = 1536;  // 128 row words, then up to 256 query words
 constexpr uint32_t kScaleBase = 2 * kFp8MaxWidth;
 constexpr size_t kMaxSmem = 232448;
-constexpr size_t kTailBytes = kScaleSlots * kSlotBytes + 512;  // scale slots and barriers
+constexpr size_t kTailBytes = kScaleSlots * kSlotBytes + 1024;  // scale slots, barriers, tiles
 constexpr int kMaxStages = 12;
+constexpr int kTileSlots = 8;  // most tiles on their way
 
+static_assert(2 * kMaxStages + 3 * kScaleSlots + 4 + 2 * kTileSlots + 1 <= 64, "barriers");
 static_assert(kScaleBase + kScaleSlots * kSlotCols <= kTmemCols, "TMEM columns");
 
 __host__ __device__ constexpr size_t stage_bytes(int width) { return kRowBytes + (size_t)width / 2 * 128; }
 
-// One tile: rows [row, row + rows) against queries [query, query + queries).
+// One tile: rows [row, row + rows) against queries [query, query + queries), results from column `col`.
 struct Tile {
-  int64_t row, query;
-  int64_t col;  // column of the first row's results
+  uint32_t row, query, col;  // below 2^31
   int rows, queries;
-  int width;    // MMA N: queries rounded up to 32
+  int width;  // MMA N: queries rounded up to 32; 0: no more tiles
 };
+__device__ __forceinline__ void pack_tile(const Tile& t, uint64_t& x, uint64_t& y) {
+  x = (uint64_t)t.row << 32 | t.query;
+  y = (uint64_t)t.col << 32 | (uint32_t)t.rows << 20 | (uint32_t)t.queries << 10 | (uint32_t)t.width;
+}
+__device__ __forceinline__ Tile unpack_tile(uint64_t x, uint64_t y) {
+  const uint32_t v = (uint32_t)y;
+  return Tile{(uint32_t)(x >> 32), (uint32_t)x, (uint32_t)(y >> 32), (int)(v >> 20), (int)(v >> 10 & 1023), (int)(v & 1023)};
+}
 
-// The tiles of a work unit, in order, from number `p` of its range to before `end`.  One group: tile p
-// is (row tile p / query_tiles, query tile p % query_tiles), and the clusters take tiles in turn, so
-// that they work side by side (results of one query in neighbouring DRAM pages).  Several groups:
-// each cluster takes a run of consecutive tiles, so that stepping from group to group stays cheap.
-struct Walk {
+// Tile (rt, qt) of an ungrouped product; all load queries by boxes of half the width.
+__device__ __forceinline__ Tile tile_at(const Fp8ScoreArgs& a, uint32_t rt, uint32_t qt) {
+  Tile x;
+  x.row = x.col = rt * (uint32_t)a.tile_rows;
+  x.query = qt * (uint32_t)a.width;
+  const int64_t rows = a.nrows - x.row, queries = a.nq - x.query;
+  x.rows = rows < a.tile_rows ? (int)rows : a.tile_rows;
+  x.queries = queries < a.width ? (int)queries : a.width;
+  x.width = a.width;
+  return x;
+}
+
+// Finds tiles by number, in ascending order, with a whole warp.  One group: tile p is (row tile
+// p / query_tiles, query tile p % query_tiles).
+struct Finder {
   const Fp8ScoreArgs& a;
   Fp8Group g;
-  int64_t p, end, step;
-  int64_t group;   // current group (groups only)
-  int64_t rt, qt;  // row and query tile within it
-  int64_t step_rt, step_qt;
-  __device__ __forceinline__ Walk(const Fp8ScoreArgs& args, int64_t unit, int64_t units) : a(args), group(0) {
+  int64_t group, first, tiles;  // current group, the tiles before it, all tiles
+  __device__ __forceinline__ explicit Finder(const Fp8ScoreArgs& args) : a(args), group(-1), first(0) {
+    tiles = a.groups.row_off ? a.groups.tile_off[a.groups.groups] : a.tiles;
+  }
+  static __device__ __forceinline__ int64_t divide(int64_t x, int64_t by) {
+    return ((uint64_t)x | (uint64_t)by) >> 32 ? x / by : (int64_t)((uint32_t)x / (uint32_t)by);
+  }
+  __device__ __forceinline__ Tile find(int64_t p) {
+    const int lane = threadIdx.x & 31;
+    Tile x{0, 0, 0, 0, 0, 0};
     if (!a.groups.row_off) {
-      g.row0 = g.query0 = 0;
-      g.nrows = a.nrows;
-      g.nqueries = a.nq;
-      g.query_tiles = a.query_tiles;
-      g.width = a.width;
-      p = unit;
-      end = a.tiles;
-      step = units;
-      rt = p / a.query_tiles;
-      qt = p % a.query_tiles;
-      step_rt = units / a.query_tiles;
-      step_qt = units % a.query_tiles;
-      return;
+      if (p >= tiles) return x;
+      const int64_t rt = divide(p, a.query_tiles);
+      return tile_at(a, (uint32_t)rt, (uint32_t)(p - rt * a.query_tiles));
     }
-    const int64_t total = a.groups.tile_off[a.groups.groups];
-    p = total * unit / units;
-    end = total * (unit + 1) / units;
-    step = step_qt = 1;
-    step_rt = rt = qt = 0;
-    if (p >= end) return;
-    int64_t lo = 0, hi = a.groups.groups;  // tile_off[lo] <= p < tile_off[hi]; 32 places tried at once
+    const int64_t* off = a.groups.tile_off;
+    int64_t lo = group < 0 ? 0 : group, hi = a.groups.groups;  // off[lo] <= p < off[hi]
+    int64_t by = 1;  // usually within the next 32 groups; else 32 places of the rest at a time
     while (hi - lo > 1) {
-      const int64_t by = (hi - lo + 31) >> 5;
-      const int64_t at = lo + by * ((threadIdx.x & 31) + 1);
-      const int k = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && a.groups.tile_off[at] <= p));
+      const int64_t at = lo + by * (lane + 1);
+      const int k = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && off[at] <= p));
       lo += by * k;
-      if (lo + by < hi) hi = lo + by;
+      if (k < 32 && lo + by < hi) hi = lo + by;
+      by = (hi - lo + 31) >> 5;
     }
-    group = lo;
-    g = fp8_group(a.groups, lo);
-    const int64_t t = p - a.groups.tile_off[lo];
-    rt = t / (g.query_tiles > 0 ? g.query_tiles : 1);
-    qt = t - rt * g.query_tiles;
-  }
-  __device__ __forceinline__ bool more() const { return p < end; }
-  __device__ __forceinline__ int64_t count() const { return p < end ? (end - p + step - 1) / step : 0; }
-  __device__ __forceinline__ void next() {
-    p += step;
-    qt += step_qt;
-    rt += step_rt;
-    if (qt >= g.query_tiles) {
-      qt -= g.query_tiles;
-      rt++;
+    if (lo != group) {
+      group = lo;
+      first = off[lo];
+      g = fp8_group(a.groups, lo);
     }
-    if (a.groups.row_off && rt * 256 >= g.nrows && p < end) {  // on to the next group that has tiles
-      do {
-        if (group + 1 >= a.groups.groups) {  // only if the offsets changed during the call
-          end = p;
-          return;
-        }
-        group++;
-        g = fp8_group(a.groups, group);
-      } while (g.tiles == 0);
-      rt = qt = 0;
-    }
-  }
-  __device__ __forceinline__ Tile tile() const {
-    Tile x;
-    x.row = g.row0 + rt * 256;
-    x.col = a.groups.row_off ? rt * 256 : x.row;
-    const int64_t rl = g.nrows - rt * 256;
-    x.rows = rl < 256 ? (int)rl : 256;
-    x.query = g.query0 + qt * g.width;
-    const int64_t ql = g.nqueries - qt * g.width;
-    x.queries = ql < g.width ? (int)(ql < 0 ? 0 : ql) : g.width;
-    // ungrouped tiles all load queries by boxes of half the width
-    x.width = !a.groups.row_off ? a.width : x.queries > 0 ? (x.queries + 31) / 32 * 32 : 32;
+    const int64_t t = p - first;
+    if (p >= tiles || g.query_tiles <= 0) return x;
+    const int64_t rt = divide(t, g.query_tiles), qt = t - rt * g.query_tiles;
+    const int64_t rows = g.nrows - rt * a.tile_rows, queries = g.nqueries - qt * g.width;
+    if (rows <= 0 || queries <= 0) return x;  // only if the offsets changed during the call
+    x.col = (uint32_t)(rt * a.tile_rows);
+    x.row = (uint32_t)(g.row0 + x.col);
+    x.query = (uint32_t)(g.query0 + qt * g.width);
+    x.rows = rows < a.tile_rows ? (int)rows : a.tile_rows;
+    x.queries = queries < g.width ? (int)queries : g.width;
+    x.width = (x.queries + 31) / 32 * 32;
     return x;
   }
 };
@@ -184,8 +179,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* sempty = sfull + kScaleSlots;
   uint64_t* tfull = sempty + kScaleSlots;
   uint64_t* tempty = tfull + 2;
-  uint64_t* drained = tempty + 2;
-  uint32_t* tmem_slot = (uint32_t*)(drained + 1);
+  uint64_t* nfull = tempty + 2;
+  uint64_t* nempty = nfull + kTileSlots;
+  uint64_t* drained = nempty + kTileSlots;
+  uint64_t* tile_slots = full + 64;  // 16-byte aligned
+  uint32_t* tmem_slot = (uint32_t*)(tile_slots + 2 * kTileSlots);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -207,6 +205,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tfull[b], 1);
       mbar_init(&tempty[b], 16);  // eight epilogue warps of each CTA
     }
+    for (int s = 0; s < kTileSlots; s++) {
+      mbar_init(&nfull[s], 1);    // the leader's tile warp
+      mbar_init(&nempty[s], 16);  // a stored tile has been read by every role before: the epilogue warps
+    }
     mbar_init(drained, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -219,20 +221,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // The launch before this one wrote the encoded queries, the groups' tile counts or both.
-  if (a.wait_first) asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  Walk walk(a, unit, units);
-  const bool any = walk.more();
+  // The launch before this one wrote the encoded queries, the groups' tile counts and the counter of
+  // tiles: every role waits for it where it needs them, and once in any case.
+  const bool grouped = a.groups.row_off != nullptr;
+  bool waited = !a.wait_first;
+  auto wait_for_prep = [&]() {
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    waited = true;
+  };
+  if (grouped) wait_for_prep();
 
   auto give_up = [&]() {
     *abort_flag = 1;
     record_error(a.err, kDevWaitTimeout);
   };
+  // Each role takes the tiles in order; false: no more, or given up.  Without groups a cluster's first
+  // tile is its number and known at once.
+  int nslot = 0;
+  uint32_t nphase = 0;
+  bool first_tile = !grouped;
+  const bool only_tile = !grouped && a.tiles <= units;
+  auto next_tile = [&](Tile& t) {
+    if (first_tile) {
+      first_tile = false;
+      const uint32_t rt = (uint32_t)unit / (uint32_t)a.query_tiles, qt = (uint32_t)unit - rt * (uint32_t)a.query_tiles;
+      t = tile_at(a, rt, qt);
+      return true;
+    }
+    if (only_tile) return false;
+    if (*abort_flag || !mbar_wait(&nfull[nslot], nphase, a.timeout_ns, abort_flag)) {
+      give_up();
+      return false;
+    }
+    const volatile uint64_t* v = tile_slots + 2 * nslot;
+    t = unpack_tile(v[0], v[1]);
+    if (++nslot == a.tile_slots) {
+      nslot = 0;
+      nphase ^= 1u;
+    }
+    return t.width != 0;
+  };
 
   if (warp == 0 || warp == 6) {
     // ---------------- TMA: warp 0 the stored rows, warp 6 the queries
-    if (any && elect_one()) {
+    if (elect_one()) {
       const bool rows = warp == 0;
       if (rows) prefetch_tmap(&maps.rows);
       else prefetch_tmap(&maps.queries[0]);
@@ -241,10 +273,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t full0 = mapa_shared(smem_addr(&full[0]), 0);
       int stage = 0;
       uint32_t phase = 0;
-      for (; walk.more() && !*abort_flag; walk.next()) {
-        const Tile t = walk.tile();
+      const int box_rows = a.tile_rows >> 1;
+      if (!rows) wait_for_prep();
+      Tile t;
+      while (next_tile(t)) {
         const int half = t.width >> 1;  // query rows of this CTA
-        const int32_t y0 = rows ? (int32_t)t.row + (int)rank * 128 : (int32_t)t.query + (int)rank * half;
+        const int32_t y0 = rows ? (int32_t)t.row + (int)rank * box_rows : (int32_t)t.query + (int)rank * half;
         for (int kc = 0; kc < a.kchunks; kc++) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, a.timeout_ns, abort_flag)) {
             give_up();
@@ -253,9 +287,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* s = stages + stage * stage_size;
           const uint32_t bar = full0 + (uint32_t)(stage * 8);
           if (rows) {
-            if (leader) mbar_arrive_expect_tx(&full[stage], 2u * (uint32_t)stage_bytes(t.width));
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2u * 128u * (uint32_t)(box_rows + half));
             tma_load_2d_pair(s, &maps.rows, bar, kc * 128, y0, policy);
-          } else if (!a.groups.row_off) {
+          } else if (!grouped) {
             tma_load_2d_pair(s + kRowBytes, &maps.queries[0], bar, kc * 128, y0, policy);
           } else {
             int32_t y = y0;
@@ -284,12 +318,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (leader && any && elect_one()) {
+    if (leader && elect_one()) {
       int stage = 0, slot = 0;
       uint32_t phase = 0, sphase = 0;
-      uint32_t li = 0;
-      for (; walk.more() && !*abort_flag; walk.next(), li++) {
-        const Tile t = walk.tile();
+      Tile t;
+      for (uint32_t li = 0; next_tile(t); li++) {
         const int acc = (int)(li & 1);
         if (!mbar_wait(&tempty[acc], ((li >> 1) & 1u) ^ 1u, a.timeout_ns, abort_flag)) {
           give_up();
@@ -354,14 +387,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     using T = typename Out<kType>::T;
     const int quarter = warp & 3;
     const int first = (warp >> 2 & 1) * 32;  // this warp's 32-query groups: every other one
-    const int my_row = (int)rank * 128 + quarter * 32 + lane;
-    const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0);
-    uint32_t li = 0;
-    for (; walk.more(); walk.next(), li++) {
-      const Tile t = walk.tile();
+    const int half_rows = a.tile_rows >> 1;
+    const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0), nempty0 = mapa_shared(smem_addr(&nempty[0]), 0);
+    for (uint32_t li = 0;; li++) {
+      Tile t;
+      const bool sent = !first_tile;  // by the tile warp, in slot nslot
+      const uint32_t nempty_bar = nempty0 + (uint32_t)(nslot * 8);
+      if (!__all_sync(0xFFFFFFFFu, next_tile(t))) break;
       const int acc = (int)(li & 1);
-      const bool row_in = my_row < t.rows;
-      T* o = (T*)a.out + (t.query + first) * a.ldo + t.col + my_row;
+      // this warp's rows of the tile
+      int rows = t.rows - (int)rank * half_rows;
+      rows = (rows < half_rows ? rows : half_rows) - quarter * 32;
+      T* o = (T*)a.out + (int64_t)(t.query + first) * a.ldo + t.col + (int)rank * half_rows + quarter * 32;
       const bool ok = !*abort_flag && mbar_wait(&tfull[acc], (li >> 1) & 1u, a.timeout_ns, abort_flag);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         if (lane == 0) give_up();
@@ -375,26 +412,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_32x32b_x32(taddr + (uint32_t)c0, v);
         tmem_ld_wait_v(v);
         const int lim = t.queries - c0;
-        if (row_in) {
+        if (lane < rows) {
+          T* at = o + lane;
           if (lim >= 32) {
 #pragma unroll
             for (int j = 0; j < 32; j++) {
-              *o = Out<kType>::of(v[j]);
-              o += a.ldo;
+              *at = Out<kType>::of(v[j]);
+              at += a.ldo;
             }
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j++) {
-              if (j < lim) *o = Out<kType>::of(v[j]);
-              o += a.ldo;
+              if (j < lim) *at = Out<kType>::of(v[j]);
+              at += a.ldo;
             }
           }
-          o += 32 * a.ldo;
         }
+        o += 64 * a.ldo;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + (uint32_t)(acc * 8));  // the leader issues the next MMA
+      if (lane == 0) {
+        mbar_arrive_cluster_relaxed(tempty0 + (uint32_t)(acc * 8));  // the leader issues the next MMA
+        if (sent) mbar_arrive_cluster_relaxed(nempty_bar);
+      }
     }
   } else if (warp < 5) {
     // ---------------- scales: warp 2 the CTA's 128 rows, warps 3 and 4 the tile's queries 0-127 and
@@ -405,16 +446,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int slots_per_tile = (a.kchunks + 3) >> 2;
     int slot = 0;
     uint32_t sphase = 0;
-    for (; walk.more(); walk.next()) {
-      const Tile t = walk.tile();
-      const int64_t first = (part == 0 ? t.row + (int)rank * 128 : t.query + (part - 1) * 128) + lane;
-      const int count = part == 0 ? 128 : t.width - (part - 1) * 128;
+    if (part > 0) wait_for_prep();
+    Tile t;
+    while (__all_sync(0xFFFFFFFFu, next_tile(t))) {
+      const int64_t first = (part == 0 ? t.row + rank * (uint32_t)(a.tile_rows >> 1) : t.query + (uint32_t)(part - 1) * 128u) + lane;
+      const int count = part == 0 ? a.tile_rows >> 1 : t.width - (part - 1) * 128;
       const uint8_t* at[4];
       bool in[4];
 #pragma unroll
       for (int c = 0; c < 4; c++) {
         const int64_t row = first + c * 32;
-        in[c] = c * 32 < count && row < limit;
+        in[c] = c * 32 + lane < count && row < limit;
         at[c] = in[c] ? src + row * (4 * (int64_t)a.scale_words) : src;
       }
       bool ok = true;
@@ -437,25 +479,62 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 5 && any && elect_one()) {
+  } else if (warp == 5) {
     // ---------------- slots that have landed go to the leader's MMA thread
-    const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
-    int slot = 0;
-    uint32_t sphase = 0;
-    for (int64_t left = walk.count() * ((a.kchunks + 3) >> 2); left > 0; left--) {
-      if (*abort_flag || !mbar_wait(&landed[slot], sphase, a.timeout_ns, abort_flag)) {
-        give_up();
+    if (elect_one()) {
+      const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
+      int slot = 0;
+      uint32_t sphase = 0;
+      Tile t;
+      while (next_tile(t)) {
+        for (int w = (a.kchunks + 3) >> 2; w > 0; w--) {
+          if (!mbar_wait(&landed[slot], sphase, a.timeout_ns, abort_flag)) {
+            give_up();
+            break;
+          }
+          fence_proxy_async();
+          mbar_arrive_pair(sfull0 + (uint32_t)(slot * 8));
+          if (++slot == kScaleSlots) {
+            slot = 0;
+            sphase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (leader && !only_tile) {
+    // ---------------- warp 7: tiles, to the same place in both CTAs
+    if (grouped || a.next_tile) wait_for_prep();
+    Finder finder(a);
+    const uint32_t at[2] = {mapa_shared(smem_addr(tile_slots), 0), mapa_shared(smem_addr(tile_slots), 1)};
+    const uint32_t bar[2] = {mapa_shared(smem_addr(nfull), 0), mapa_shared(smem_addr(nfull), 1)};
+    int64_t p = unit;
+    bool own = grouped;  // the first number is the cluster's own, and without groups known to every role
+    for (int width = 1; width != 0; own = false) {
+      if (!own && a.next_tile) {
+        unsigned long long n = 0;
+        if (lane == 0) n = atomicAdd(a.next_tile, 1ull);
+        p = units + (int64_t)__shfl_sync(0xFFFFFFFFu, n, 0);
+      } else if (!own) {
+        p += units;
+      }
+      const Tile t = finder.find(p);
+      width = t.width;
+      const bool ok = mbar_wait(&nempty[nslot], nphase ^ 1u, a.timeout_ns, abort_flag);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        if (lane == 0) give_up();
         break;
       }
-      fence_proxy_async();
-      mbar_arrive_pair(sfull0 + (uint32_t)(slot * 8));
-      if (++slot == kScaleSlots) {
-        slot = 0;
-        sphase ^= 1u;
+      uint64_t x, y;
+      pack_tile(t, x, y);
+      if (lane < 2) store_cluster_16(at[lane] + (uint32_t)nslot * 16u, bar[lane] + (uint32_t)nslot * 8u, x, y);
+      if (++nslot == a.tile_slots) {
+        nslot = 0;
+        nphase ^= 1u;
       }
     }
   }
 
+  wait_for_prep();
   tc_fence_before();
   cluster_sync();  // the pair's MMAs, loads and epilogues are done with TMEM and shared memory
   if (warp == 1) {
@@ -496,22 +575,32 @@ cudaError_t launch_typed(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, 
 
 }  // namespace
 
+Fp8Tiling fp8_tiling(int64_t nrows, int64_t nq, int64_t groups, int num_sms) {
+  Fp8Tiling t{};
+  t.tile_rows = 256;
+  t.query_tiles = (int)((nq + kFp8MaxWidth - 1) / kFp8MaxWidth);
+  if (groups > 0) {  // the widest tile any group can have
+    t.width = (int)(nq < kFp8MaxWidth ? (nq + 31) / 32 * 32 : kFp8MaxWidth);
+    return t;
+  }
+  // equal tiles of at most kFp8MaxWidth queries
+  t.width = (int)(((nq + t.query_tiles - 1) / t.query_tiles + 31) / 32 * 32);
+  t.tiles = (nrows + t.tile_rows - 1) / t.tile_rows * t.query_tiles;
+  return t;
+}
+
 cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& args, int out_type, int num_sms, bool after_prep,
                               cudaStream_t st) {
   Fp8ScoreArgs a = args;
-  const int64_t qt = (a.nq + kFp8MaxWidth - 1) / kFp8MaxWidth;
   int64_t units = num_sms / 2;
-  if (a.groups.row_off) {
-    a.width = (int)(a.nq < kFp8MaxWidth ? (a.nq + 31) / 32 * 32 : kFp8MaxWidth);  // widest possible tile
-  } else {
-    a.query_tiles = (int)qt;
-    a.width = fp8_query_width(a.nq);
-    a.tiles = (a.nrows + 255) / 256 * qt;
-    if (units > a.tiles) units = a.tiles;
-  }
+  if (!a.groups.row_off && units > a.tiles) units = a.tiles;
   if (units < 1) units = 1;
   a.stages = (int)((kMaxSmem - 1024 - kTailBytes) / stage_bytes(a.width));
   if (a.stages > kMaxStages) a.stages = kMaxStages;
+  // Tiles on their way in a cluster: one multiplied, one stored, and those that the stages can hold
+  // beyond (fewer leave the end of the work better shared out).
+  a.tile_slots = 2 + (a.stages + a.kchunks - 1) / a.kchunks;
+  if (a.tile_slots > kTileSlots) a.tile_slots = kTileSlots;
   a.wait_first = after_prep;
   const size_t smem = 1024 + a.stages * stage_bytes(a.width) + kTailBytes;
   switch (out_type) {

@@ -230,6 +230,14 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// 16 bytes into the shared memory of a CTA of the cluster, counted on a barrier of that CTA (whose
+// phase also gets this thread's arrival).
+__device__ __forceinline__ void store_cluster_16(uint32_t dst, uint32_t bar, uint64_t x, uint64_t y) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], 16;" ::"r"(bar) : "memory");
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(dst), "l"(x),
+               "l"(y), "r"(bar)
+               : "memory");
+}
 // 4-byte copy from global to shared memory (zero when !valid), and an arrival on `bar` when all of
 // this thread's copies so far have landed.
 __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, bool valid) {
