@@ -8,14 +8,17 @@
 // byte, and the tensor cores apply it inside the product (fp8_scores.cu).  A block that holds a
 // NaN or an infinity is NaN throughout: scale byte 255, codes 0x7f.
 //
-// Both kernels stream: per row they move dim elements and pitch(dim) codes + scales.  One warp takes
-// up to kWords x 4 blocks of one row, 4 elements a lane and block: their loads are in flight
-// together, every access of the warp is consecutive, and four blocks' scales make one 32-bit word.
+// Both kernels stream: per row they move dim elements and pitch(dim) codes + scales.
+//   write  8 lanes take a block, 16 elements each in pieces of 16 (or 8) bytes, so that both sides are
+//          consecutive, the block's maximum is three shuffles away, and rows of any number of blocks
+//          fill the warps.  (A prefetched next block costs more in resident warps than it hides.)
+//   read   one warp takes up to 8 blocks of a row, 4 elements a lane and block, so that the wider
+//          side, its stores, is consecutive.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include <cstring>
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/vx.h"
@@ -35,12 +38,6 @@ __device__ __forceinline__ int64_t slot_at(const void* slots, int slot_bytes, in
 
 // ---------------------------------------------------------------- element types
 template <class T>
-__device__ __forceinline__ float to_f32(T v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
-  else return __bfloat162float(v);
-}
-template <class T>
 __device__ __forceinline__ T from_f32(float v) {
   if constexpr (sizeof(T) == 4) return v;
   else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
@@ -50,30 +47,53 @@ template <class T>
 struct alignas(4 * sizeof(T)) Four {
   T v[4];
 };
-// Four elements that this kernel reads once.
-template <class T>
-__device__ __forceinline__ Four<T> load_four(const T* p) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 f = __ldcs(reinterpret_cast<const float4*>(p));
-    return Four<T>{{f.x, f.y, f.z, f.w}};
+// Elements k .. k + kE - 1 of a row as they are, zero from dim on; kVec: by one load where all exist.
+template <class T, int kE, bool kVec>
+__device__ __forceinline__ void load_piece(const T* row, int k, int dim, uint32_t* r) {
+  constexpr int kWords = kE * (int)sizeof(T) / 4;
+  if (kVec && k + kE <= dim) {
+    if constexpr (kWords == 4) {
+      const uint4 u = __ldcs((const uint4*)(row + k));
+      r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
+    } else {
+      const uint2 u = __ldcs((const uint2*)(row + k));
+      r[0] = u.x, r[1] = u.y;
+    }
   } else {
-    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(p));
-    Four<T> f;
-    memcpy(&f, &u, 8);
-    return f;
+#pragma unroll
+    for (int i = 0; i < kWords; i++) {
+      if constexpr (sizeof(T) == 4) {
+        r[i] = k + i < dim ? __float_as_uint(row[k + i]) : 0u;
+      } else {
+        const uint16_t* x = (const uint16_t*)row + k + 2 * i;
+        r[i] = k + 2 * i < dim ? x[0] : 0u;
+        if (k + 2 * i + 1 < dim) r[i] |= (uint32_t)x[1] << 16;
+      }
+    }
   }
 }
+// Element i of a piece.
+template <class T>
+__device__ __forceinline__ float element(const uint32_t* r, int i) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r[i]);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return __uint_as_float(i & 1 ? r[i / 2] & 0xFFFF0000u : r[i / 2] << 16);
+  else return __half2float(__ushort_as_half((unsigned short)(i & 1 ? r[i / 2] >> 16 : r[i / 2] & 0xFFFFu)));
+}
 
-// Elements k .. k + 3 of a row; zero from dim on.
-template <class T, bool kVec>
-__device__ __forceinline__ void load4(const T* row, int k, int dim, float (&x)[4]) {
-  if (kVec && k + 4 <= dim) {
-    const Four<T> f = load_four<T>(row + k);
+// Bits of the largest magnitude of 16 elements, as float32's.
+template <class T>
+__device__ __forceinline__ uint32_t largest(const uint32_t (&r)[4 * sizeof(T)]) {
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = to_f32<T>(f.v[i]);
-  } else {
+    for (int i = 0; i < 16; i++) m = max(m, r[i] & 0x7FFFFFFFu);
+    return m;
+  } else {  // magnitudes of 16 bits order as integers
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = k + i < dim ? to_f32<T>(row[k + i]) : 0.0f;
+    for (int i = 0; i < 8; i++) m = __vmaxu2(m, r[i] & 0x7FFF7FFFu);
+    m = max(m >> 16, m & 0xFFFFu);
+    return __float_as_uint(element<T>(&m, 0));
   }
 }
 
@@ -106,72 +126,89 @@ __global__ void owner_kernel(const void* slots, int slot_bytes, int64_t n, int64
 }
 
 // ---------------------------------------------------------------- write
-// Blocks of 8 warps; block b takes rows 8 (b / parts) + warp, part b % parts of their words.
-// kGroups: block 0 counts a grouped product's tiles instead.
-template <class T, bool kVec, int kWords, bool kGroups>
-__global__ void __launch_bounds__(kThreads) fp8_write_kernel(const Fp8WriteArgs a, const Fp8Groups groups,
-                                                             unsigned long long* counter, uint32_t parts) {
+// Work is counted in blocks of 128 dimensions, row after row; a CTA takes kRun of them at a time and
+// goes on gridDim.x runs further.  kGroups: the last CTA counts a grouped product's tiles instead.
+constexpr int kRun = kThreads / 8;
+
+template <class T, int kE, bool kVec, bool kGroups>
+__global__ void __launch_bounds__(kThreads, 6) fp8_write_kernel(const Fp8WriteArgs a, const Fp8Groups groups,
+                                                             unsigned long long* counter) {
   launch_dependents();
   if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;
-  uint32_t block = blockIdx.x;
+  const uint32_t ctas = gridDim.x - (kGroups ? 1 : 0);
   if constexpr (kGroups) {
-    if (block == 0) {
+    if (blockIdx.x == ctas) {
       fp8_count_tiles<kThreads>(groups);
       return;
     }
-    block--;
   }
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)(block / parts) * (kThreads / 32) + (threadIdx.x >> 5);
-  const int first = (int)(block % parts) * kWords * 4;  // first block of the row's
-  const int nb = (a.dim + kFp8Block - 1) / kFp8Block;
-  const T* x = (const T*)a.rows + row * a.stride;
-  float v[kWords * 4][4];
-  int64_t slot = -1;
-  if (row < a.n) {
+  constexpr int kPieces = 16 / kE, kWords = kE * (int)sizeof(T) / 4;
+  const int part = threadIdx.x & 7;
+  const uint32_t nb = (uint32_t)(a.dim + kFp8Block - 1) / kFp8Block;
+  const uint32_t scale_pitch = (nb + 3) / 4 * 4;
+  const uint64_t begin = (uint64_t)blockIdx.x * kRun + (threadIdx.x >> 3), step = (uint64_t)ctas * kRun;
+  const auto divide = [nb](uint64_t x) { return x >> 32 ? x / nb : (uint64_t)((uint32_t)x / nb); };
+  int64_t row = (int64_t)divide(begin);
+  uint32_t at = (uint32_t)(begin - (uint64_t)row * nb);  // block within the row
+  const int64_t step_row = (int64_t)divide(step);
+  const uint32_t step_at = (uint32_t)(step - (uint64_t)step_row * nb);
+
+  bool first = true;
+  for (; __any_sync(0xFFFFFFFFu, row < a.n); first = false) {
+    uint32_t r[kPieces * kWords];
+    int64_t slot = -1;
+    if (row < a.n) {
+      const T* x = (const T*)a.rows + row * a.stride;
 #pragma unroll
-    for (int j = 0; j < kWords * 4; j++) load4<T, kVec>(x, (first + j) * kFp8Block + lane * 4, a.dim, v[j]);
-    slot = a.slots ? slot_at(a.slots, a.slot_bytes, row) : a.first + row;
-  }
-  if (a.owner) wait_for_launch_before();  // every thread: no block ends before the launches before it
-  if (slot < 0 || slot >= a.capacity) return;
-  if (a.slots) {
-    if (a.owner) {
-      if (__ldcg(a.owner + slot) != (int32_t)row) return;
-    } else {
-      bool later = false;
-      for (int64_t j = row + 1 + lane; j < a.n; j += 32) later |= slot_at(a.slots, a.slot_bytes, j) == slot;
-      if (__any_sync(0xFFFFFFFFu, later)) return;
+      for (int i = 0; i < kPieces; i++)
+        load_piece<T, kE, kVec>(x, (int)at * kFp8Block + (i * 8 + part) * kE, a.dim, r + i * kWords);
+      slot = a.slots ? slot_at(a.slots, a.slot_bytes, row) : a.first + row;
+      if (slot >= a.capacity) slot = -1;
     }
-  }
-  uint8_t* codes = a.codes + slot * ((int64_t)nb * kFp8Block);
-  uint8_t* scales = a.scales + slot * (int64_t)((nb + 3) / 4 * 4);
-#pragma unroll
-  for (int w = 0; w < kWords; w++) {
-    if (first + 4 * w >= nb) break;
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float(&y)[4] = v[4 * w + j];
-      const int k = first + 4 * w + j;
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(y[i]) & 0x7FFFFFFFu);
-      m = __reduce_max_sync(0xFFFFFFFFu, m);
-      if (k >= nb) break;
-      const int b = scale_byte(m);
-      word |= (uint32_t)b << (8 * j);
-      uint32_t c = 0x7F7F7F7Fu;
-      if (b != 255) {
-        const float inv = __uint_as_float((uint32_t)(254 - b) << 23);  // 2^(127 - b), b <= 247
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0] * inv, y[1] * inv), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2] * inv, y[3] * inv), __NV_SATFINITE, __NV_E4M3);
-        c = lo | (hi << 16);
+    if (a.owner && first) wait_for_launch_before();
+    bool keep = slot >= 0;
+    if (keep && a.slots) {
+      if (a.owner) {
+        keep = __ldcg(a.owner + slot) == (int32_t)row;
+      } else {
+        for (int64_t j = row + 1; j < a.n; j++) keep &= slot_at(a.slots, a.slot_bytes, j) != slot;
       }
-      *(uint32_t*)(codes + k * kFp8Block + lane * 4) = c;
     }
-    if (lane == 0) *(uint32_t*)(scales + first + 4 * w) = word;
+    uint32_t m = keep ? largest<T>(r) : 0u;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (keep) {
+      const int b = scale_byte(m);
+      const float inv = __uint_as_float((uint32_t)(254 - (b == 255 ? 0 : b)) << 23);  // 2^(127 - b), b <= 247
+      uint8_t* codes = a.codes + slot * ((int64_t)nb * kFp8Block) + at * kFp8Block + part * kE;
+#pragma unroll
+      for (int i = 0; i < kPieces; i++) {
+        uint32_t c[kE / 4];
+#pragma unroll
+        for (int q = 0; q < kE / 4; q++) {
+          const uint32_t* x = r + i * kWords;
+          const float2 lo = make_float2(element<T>(x, 4 * q) * inv, element<T>(x, 4 * q + 1) * inv);
+          const float2 hi = make_float2(element<T>(x, 4 * q + 2) * inv, element<T>(x, 4 * q + 3) * inv);
+          c[q] = (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
+                 (uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16;
+          if (b == 255) c[q] = 0x7F7F7F7Fu;
+        }
+        if constexpr (kE == 8) *(uint2*)(codes + i * 64) = make_uint2(c[0], c[1]);
+        else *(uint32_t*)(codes + i * 32) = c[0];
+      }
+      // the scale's byte, and after the last block's the zeros up to a word
+      uint8_t* scale = a.scales + slot * (int64_t)scale_pitch + at;
+      if (part == 0) *scale = (uint8_t)b;
+      else if (at + 1 == nb && at + part < scale_pitch) scale[part] = 0;
+    }
+    row += step_row;
+    at += step_at;
+    if (at >= nb) {
+      at -= nb;
+      row++;
+    }
   }
+  if (a.owner && first) wait_for_launch_before();  // no CTA ends before the launches before it
 }
 
 __global__ void __launch_bounds__(1024) fp8_count_tiles_kernel(const Fp8Groups groups, unsigned long long* counter) {
@@ -231,13 +268,8 @@ bool four_aligned(const void* p, int64_t stride) {
   return (uintptr_t)p % (4 * sizeof(T)) == 0 && stride % 4 == 0;
 }
 
-// Parts of a row of `words` scale words that a warp each takes, and the blocks for n rows.
+// Parts of a row of `words` scale words that a warp each takes.
 int parts_of(int words, int per) { return (words + per - 1) / per; }
-bool grid_for(int64_t n, int parts, int extra, unsigned* grid) {
-  const int64_t g = (n + kThreads / 32 - 1) / (kThreads / 32) * parts + extra;
-  *grid = (unsigned)g;
-  return g <= 0x7FFFFFFF;
-}
 
 // Launches `kern`, allowed to begin before the launch before it ends if `dependent`.
 template <class... P, class... A>
@@ -254,23 +286,35 @@ cudaError_t launch(void (*kern)(P...), unsigned grid, int threads, bool dependen
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <class T, int kWords, bool kGroups>
-cudaError_t write_words(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, int words, cudaStream_t st) {
-  const int parts = parts_of(words, kWords);
-  unsigned grid;
-  if (!grid_for(a.n, parts, kGroups ? 1 : 0, &grid)) return cudaErrorInvalidValue;
-  const bool dependent = a.owner != nullptr;
-  if (four_aligned<T>(a.rows, a.stride))
-    return launch(fp8_write_kernel<T, true, kWords, kGroups>, grid, kThreads, dependent, st, a, g, counter, (uint32_t)parts);
-  return launch(fp8_write_kernel<T, false, kWords, kGroups>, grid, kThreads, dependent, st, a, g, counter, (uint32_t)parts);
+// As many CTAs as stay on the device at once, or as there are runs of work; where that leaves each
+// more than 8 runs, CTAs of 4 that the device shares out as they end (400k x 1024 fp32: 304 us, 348 in
+// one wave; 16k x 1024 bf16: 10.8 us in one wave, 13.2 in CTAs of 4).
+template <class T, int kE, bool kVec, bool kGroups>
+cudaError_t write_variant(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, cudaStream_t st) {
+  static std::atomic<int> per_sm{0};
+  auto kern = fp8_write_kernel<T, kE, kVec, kGroups>;
+  int n = per_sm.load();
+  if (n == 0) {
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kThreads, 0);
+    if (e != cudaSuccess) return e;
+    per_sm.store(n);
+  }
+  const int64_t runs = (a.n * fp8_blocks(a.dim) + kRun - 1) / kRun;
+  const int64_t most = (int64_t)n * a.num_sms;
+  int64_t grid = runs < most ? runs : most;
+  if (runs > 8 * most) grid = (runs + 3) / 4;
+  grid += kGroups ? 1 : 0;
+  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  return launch(kern, (unsigned)grid, kThreads, a.owner != nullptr, st, a, g, counter);
 }
 
-// Rows of more than 512 dimensions: a warp takes 8 blocks (kWords 2), else 4.
 template <class T, bool kGroups>
 cudaError_t write_typed(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long long* counter, cudaStream_t st) {
-  const int words = fp8_scale_pitch(a.dim) / 4;
-  return words > 1 ? write_words<T, 2, kGroups>(a, g, counter, words, st)
-                   : write_words<T, 1, kGroups>(a, g, counter, words, st);
+  // the widest loads that every row's first element is aligned for
+  const uintptr_t bits = (uintptr_t)a.rows | (uintptr_t)(a.stride * (int64_t)sizeof(T));
+  if (bits % 16 == 0) return write_variant<T, 16 / sizeof(T), true, kGroups>(a, g, counter, st);
+  if (sizeof(T) == 2 && bits % 8 == 0) return write_variant<T, 4, true, kGroups>(a, g, counter, st);
+  return write_variant<T, 4, false, kGroups>(a, g, counter, st);
 }
 
 template <bool kGroups>
@@ -286,11 +330,11 @@ cudaError_t write_any(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned long l
 template <class T, int kWords>
 cudaError_t read_words(const Fp8ReadArgs& a, int words, cudaStream_t st) {
   const int parts = parts_of(words, kWords);
-  unsigned grid;
-  if (!grid_for(a.n, parts, 0, &grid)) return cudaErrorInvalidValue;
+  const int64_t grid = (a.n + kThreads / 32 - 1) / (kThreads / 32) * parts;
+  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
   if (four_aligned<T>(a.out, a.stride))
-    return launch(fp8_read_kernel<T, true, kWords>, grid, kThreads, false, st, a, (uint32_t)parts);
-  return launch(fp8_read_kernel<T, false, kWords>, grid, kThreads, false, st, a, (uint32_t)parts);
+    return launch(fp8_read_kernel<T, true, kWords>, (unsigned)grid, kThreads, false, st, a, (uint32_t)parts);
+  return launch(fp8_read_kernel<T, false, kWords>, (unsigned)grid, kThreads, false, st, a, (uint32_t)parts);
 }
 
 template <class T>

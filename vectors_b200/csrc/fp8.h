@@ -43,6 +43,7 @@ struct Fp8WriteArgs {
   uint8_t* scales;
   int64_t capacity;
   int32_t* owner;  // [capacity] scratch; needed for more than kFp8DirectSlots rows with slots
+  int num_sms;
 };
 
 struct Fp8ReadArgs {

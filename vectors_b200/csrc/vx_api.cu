@@ -2705,6 +2705,7 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
       w.n = w.capacity = q.nq;
       w.dim = dim;
       w.stride = q.stride;
+      w.num_sms = dev->sms;
       w.codes = buf + q_at;
       w.scales = w.codes + (size_t)q.nq * pitch;
       q_codes = w.codes;
@@ -2758,7 +2759,7 @@ int vx_fp8_write_device(int32_t device, const void* rows, int32_t type, int64_t 
     DeviceScope here(device);
     cudaStream_t st = (cudaStream_t)stream;
     Scratch S(st);
-    Fp8WriteArgs a{rows, type, n, dim, row_stride, slots, slot_bytes, first, codes, scales, capacity, nullptr};
+    Fp8WriteArgs a{rows, type, n, dim, row_stride, slots, slot_bytes, first, codes, scales, capacity, nullptr, dev->sms};
     if (slots && n > kFp8DirectSlots) a.owner = S.alloc<int32_t>((size_t)capacity);
     int launches = 0;
     cudaError_t e = launch_fp8_write(a, &launches, st);
