@@ -127,7 +127,7 @@ __global__ void owner_kernel(const void* slots, int slot_bytes, int64_t n, int64
 
 // ---------------------------------------------------------------- write
 // Work is counted in blocks of 128 dimensions, row after row; a CTA takes kRun of them at a time and
-// goes on gridDim.x runs further.  kGroups: the last CTA counts a grouped product's tiles instead.
+// goes on gridDim.x runs further.  kGroups: CTA 0 counts a grouped product's tiles instead.
 constexpr int kRun = kThreads / 8;
 
 template <class T, int kE, bool kVec, bool kGroups>
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 6) fp8_write_kernel(const Fp8WriteAr
   if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;
   const uint32_t ctas = gridDim.x - (kGroups ? 1 : 0);
   if constexpr (kGroups) {
-    if (blockIdx.x == ctas) {
+    if (blockIdx.x == 0) {
       fp8_count_tiles<kThreads>(groups);
       return;
     }
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 6) fp8_write_kernel(const Fp8WriteAr
   const int part = threadIdx.x & 7;
   const uint32_t nb = (uint32_t)(a.dim + kFp8Block - 1) / kFp8Block;
   const uint32_t scale_pitch = (nb + 3) / 4 * 4;
-  const uint64_t begin = (uint64_t)blockIdx.x * kRun + (threadIdx.x >> 3), step = (uint64_t)ctas * kRun;
+  const uint64_t begin = (uint64_t)(blockIdx.x - (kGroups ? 1 : 0)) * kRun + (threadIdx.x >> 3), step = (uint64_t)ctas * kRun;
   const auto divide = [nb](uint64_t x) { return x >> 32 ? x / nb : (uint64_t)((uint32_t)x / nb); };
   int64_t row = (int64_t)divide(begin);
   uint32_t at = (uint32_t)(begin - (uint64_t)row * nb);  // block within the row
@@ -300,7 +300,7 @@ cudaError_t write_variant(const Fp8WriteArgs& a, const Fp8Groups& g, unsigned lo
     per_sm.store(n);
   }
   const int64_t runs = (a.n * fp8_blocks(a.dim) + kRun - 1) / kRun;
-  const int64_t most = (int64_t)n * a.num_sms;
+  const int64_t most = (int64_t)n * a.num_sms - (kGroups ? 1 : 0);
   int64_t grid = runs < most ? runs : most;
   if (runs > 8 * most) grid = (runs + 3) / 4;
   grid += kGroups ? 1 : 0;

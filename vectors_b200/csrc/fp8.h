@@ -11,7 +11,8 @@ namespace vx {
 
 constexpr int kFp8Block = 128;        // dimensions that share a scale
 constexpr int kFp8MaxDim = 1 << 16;
-constexpr int kFp8MaxWidth = 224;     // queries of one product tile (TMEM columns per accumulator)
+constexpr int kFp8MaxWidth = 224;     // most queries of one product tile (TMEM columns per accumulator)
+constexpr int kFp8TileRows = 256;     // most stored rows of one
 // batches of at most this many rows find repeated slots by comparing slots directly (fp8.cu)
 constexpr int64_t kFp8DirectSlots = 256;
 
@@ -19,15 +20,27 @@ inline int fp8_blocks(int dim) { return (dim + kFp8Block - 1) / kFp8Block; }
 inline int fp8_code_pitch(int dim) { return fp8_blocks(dim) * kFp8Block; }  // bytes of codes per row
 inline int fp8_scale_pitch(int dim) { return (fp8_blocks(dim) + 3) / 4 * 4; }  // bytes of scales per row
 
-// A grouped product's offsets, the sizes they are clamped to, and where the tiles before each group go.
+// A grouped product's offsets, the sizes they are clamped to, and where each group's bounds and the
+// tiles before it go.
 struct Fp8Groups {
   const int64_t* row_off;    // [groups + 1]; null: one group of every row and query
   const int64_t* query_off;  // [groups + 1]
   int64_t groups;
   int64_t nrows, nq;
   int64_t max_cols;   // results kept per query (groups with more rows are cut there)
-  int tile_rows;      // stored rows of a tile
+  int4* bounds;       // [groups]
   int64_t* tile_off;  // [groups + 1]
+  ulonglong2* first;  // [firsts] the first tiles, packed (width 0: there are fewer)
+  int firsts;
+};
+
+// One tile of a product: rows [row, row + rows) against queries [query, query + queries), results from
+// column `col`.
+struct Fp8Tile {
+  uint32_t row, query, col;  // below 2^31
+  int rows, queries;
+  int width;  // MMA N: queries rounded up to 32; 0: no more tiles
+  int half;   // rows of each CTA: the leader's are the first `half`
 };
 
 struct Fp8WriteArgs {
@@ -89,11 +102,11 @@ struct Fp8ScoreArgs {
   int wait_first;
 };
 
-// The operands' tensor maps: `rows` with boxes of half a tile's rows; queries[0] with boxes of half a
-// tile's queries, or with groups queries[i] with boxes of 64 >> i rows.
+// The operands' tensor maps: rows[0] with boxes of half a tile's rows and queries[0] with boxes of half a
+// tile's queries; with groups, whose tiles differ, rows[i] and queries[i] with boxes of 128 >> i rows.
 struct Fp8Maps {
-  CUtensorMap rows;
-  CUtensorMap queries[3];
+  CUtensorMap rows[4];
+  CUtensorMap queries[4];
 };
 
 // The tiling of a product: tile sizes and, without groups, the number of tiles.

@@ -69,20 +69,7 @@ static_assert(kScaleBase + kScaleSlots * kSlotCols <= kTmemCols, "TMEM columns")
 
 __host__ __device__ constexpr size_t stage_bytes(int width) { return kRowBytes + (size_t)width / 2 * 128; }
 
-// One tile: rows [row, row + rows) against queries [query, query + queries), results from column `col`.
-struct Tile {
-  uint32_t row, query, col;  // below 2^31
-  int rows, queries;
-  int width;  // MMA N: queries rounded up to 32; 0: no more tiles
-};
-__device__ __forceinline__ void pack_tile(const Tile& t, uint64_t& x, uint64_t& y) {
-  x = (uint64_t)t.row << 32 | t.query;
-  y = (uint64_t)t.col << 32 | (uint32_t)t.rows << 20 | (uint32_t)t.queries << 10 | (uint32_t)t.width;
-}
-__device__ __forceinline__ Tile unpack_tile(uint64_t x, uint64_t y) {
-  const uint32_t v = (uint32_t)y;
-  return Tile{(uint32_t)(x >> 32), (uint32_t)x, (uint32_t)(y >> 32), (int)(v >> 20), (int)(v >> 10 & 1023), (int)(v & 1023)};
-}
+using Tile = Fp8Tile;
 
 // Tile (rt, qt) of an ungrouped product; all load queries by boxes of half the width.
 __device__ __forceinline__ Tile tile_at(const Fp8ScoreArgs& a, uint32_t rt, uint32_t qt) {
@@ -93,6 +80,7 @@ __device__ __forceinline__ Tile tile_at(const Fp8ScoreArgs& a, uint32_t rt, uint
   x.rows = rows < a.tile_rows ? (int)rows : a.tile_rows;
   x.queries = queries < a.width ? (int)queries : a.width;
   x.width = a.width;
+  x.half = a.tile_rows >> 1;
   return x;
 }
 
@@ -110,7 +98,7 @@ struct Finder {
   }
   __device__ __forceinline__ Tile find(int64_t p) {
     const int lane = threadIdx.x & 31;
-    Tile x{0, 0, 0, 0, 0, 0};
+    Tile x{0, 0, 0, 0, 0, 0, 0};
     if (!a.groups.row_off) {
       if (p >= tiles) return x;
       const int64_t rt = divide(p, a.query_tiles);
@@ -118,31 +106,30 @@ struct Finder {
     }
     const int64_t* off = a.groups.tile_off;
     int64_t lo = group < 0 ? 0 : group, hi = a.groups.groups;  // off[lo] <= p < off[hi]
-    int64_t by = 1;  // usually within the next 32 groups; else 32 places of the rest at a time
-    while (hi - lo > 1) {
-      const int64_t at = lo + by * (lane + 1);
-      const int k = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && off[at] <= p));
-      lo += by * k;
-      if (k < 32 && lo + by < hi) hi = lo + by;
-      by = (hi - lo + 31) >> 5;
+    // usually within the next 128 groups, whose offsets are looked at together; else 32 places of the
+    // rest at a time
+    int k = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t at = lo + 1 + i * 32 + lane;
+      k += __popc(__ballot_sync(0xFFFFFFFFu, at < hi && off[at] <= p));
     }
+    lo += k;
+    if (k < 128) hi = lo + 1;
+    while (hi - lo > 1) {
+      const int64_t by = (hi - lo + 31) >> 5;
+      const int64_t at = lo + by * (lane + 1);
+      k = __popc(__ballot_sync(0xFFFFFFFFu, at < hi && off[at] <= p));
+      lo += by * k;
+      if (lo + by < hi) hi = lo + by;
+    }
+    if (p >= tiles) return x;
     if (lo != group) {
       group = lo;
       first = off[lo];
-      g = fp8_group(a.groups, lo);
+      g = fp8_group(a.groups.bounds[lo]);
     }
-    const int64_t t = p - first;
-    if (p >= tiles || g.query_tiles <= 0) return x;
-    const int64_t rt = divide(t, g.query_tiles), qt = t - rt * g.query_tiles;
-    const int64_t rows = g.nrows - rt * a.tile_rows, queries = g.nqueries - qt * g.width;
-    if (rows <= 0 || queries <= 0) return x;  // only if the offsets changed during the call
-    x.col = (uint32_t)(rt * a.tile_rows);
-    x.row = (uint32_t)(g.row0 + x.col);
-    x.query = (uint32_t)(g.query0 + qt * g.width);
-    x.rows = rows < a.tile_rows ? (int)rows : a.tile_rows;
-    x.queries = queries < g.width ? (int)queries : g.width;
-    x.width = (x.queries + 31) / 32 * 32;
-    return x;
+    return fp8_group_tile(g, p - first);
   }
 };
 
@@ -190,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+  if (warp == 0 && lane < 2) prefetch_tmap(lane == 0 ? &maps.rows[0] : &maps.queries[0]);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stages; s++) {
@@ -229,26 +217,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
     waited = true;
   };
-  if (grouped) wait_for_prep();
 
   auto give_up = [&]() {
     *abort_flag = 1;
     record_error(a.err, kDevWaitTimeout);
   };
-  // Each role takes the tiles in order; false: no more, or given up.  Without groups a cluster's first
-  // tile is its number and known at once.
+  // Each role takes the tiles in order; false: no more, or given up.  A cluster's first tile is the one of
+  // its number: without groups known at once, with groups one of those that the launch before this one
+  // left.
   int nslot = 0;
   uint32_t nphase = 0;
-  bool first_tile = !grouped;
+  bool first_tile = true;
   const bool only_tile = !grouped && a.tiles <= units;
+  bool ended = false;
   auto next_tile = [&](Tile& t) {
     if (first_tile) {
       first_tile = false;
+      if (grouped) {
+        wait_for_prep();
+        const ulonglong2 v = a.groups.first[unit];
+        t = unpack_tile(v.x, v.y);
+        if (t.width == 0) ended = true;
+        return t.width != 0;
+      }
       const uint32_t rt = (uint32_t)unit / (uint32_t)a.query_tiles, qt = (uint32_t)unit - rt * (uint32_t)a.query_tiles;
       t = tile_at(a, rt, qt);
       return true;
     }
-    if (only_tile) return false;
+    if (only_tile || ended) return false;
     if (*abort_flag || !mbar_wait(&nfull[nslot], nphase, a.timeout_ns, abort_flag)) {
       give_up();
       return false;
@@ -266,39 +262,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- TMA: warp 0 the stored rows, warp 6 the queries
     if (elect_one()) {
       const bool rows = warp == 0;
-      if (rows) prefetch_tmap(&maps.rows);
-      else prefetch_tmap(&maps.queries[0]);
+      const CUtensorMap* map = rows ? maps.rows : maps.queries;
       // query tiles are read again for every row tile
       const uint64_t policy = rows ? policy_evict_normal() : policy_evict_last();
       const uint32_t full0 = mapa_shared(smem_addr(&full[0]), 0);
       int stage = 0;
       uint32_t phase = 0;
-      const int box_rows = a.tile_rows >> 1;
       if (!rows) wait_for_prep();
       Tile t;
       while (next_tile(t)) {
-        const int half = t.width >> 1;  // query rows of this CTA
-        const int32_t y0 = rows ? (int32_t)t.row + (int)rank * box_rows : (int32_t)t.query + (int)rank * half;
+        const int count = rows ? t.half : t.width >> 1;  // operand rows of this CTA
+        const int32_t y0 = (int32_t)(rows ? t.row : t.query) + (int)rank * count;
         for (int kc = 0; kc < a.kchunks; kc++) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, a.timeout_ns, abort_flag)) {
             give_up();
             break;
           }
-          uint8_t* s = stages + stage * stage_size;
+          uint8_t* s = stages + stage * stage_size + (rows ? 0 : kRowBytes);
           const uint32_t bar = full0 + (uint32_t)(stage * 8);
-          if (rows) {
-            if (leader) mbar_arrive_expect_tx(&full[stage], 2u * 128u * (uint32_t)(box_rows + half));
-            tma_load_2d_pair(s, &maps.rows, bar, kc * 128, y0, policy);
-          } else if (!grouped) {
-            tma_load_2d_pair(s + kRowBytes, &maps.queries[0], bar, kc * 128, y0, policy);
+          if (rows && leader) mbar_arrive_expect_tx(&full[stage], 2u * 128u * (uint32_t)(count + (t.width >> 1)));
+          if (!grouped) {
+            tma_load_2d_pair(s, map, bar, kc * 128, y0, policy);
           } else {
             int32_t y = y0;
-            s += kRowBytes;
 #pragma unroll
-            for (int i = 0; i < 3; i++) {  // the half's rows as boxes of 64, 32 and 16
-              const int box = 64 >> i;
-              if (half & box) {
-                tma_load_2d_pair(s, &maps.queries[i], bar, kc * 128, y, policy);
+            for (int i = 0; i < 4; i++) {  // boxes of 128, 64, 32 and 16 rows
+              const int box = 128 >> i;
+              if (count & box) {
+                tma_load_2d_pair(s, map + i, bar, kc * 128, y, policy);
                 s += box * 128;
                 y += box;
               }
@@ -321,6 +312,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (leader && elect_one()) {
       int stage = 0, slot = 0;
       uint32_t phase = 0, sphase = 0;
+      const uint64_t desc0 = sw128_kmajor_desc(smem_addr(stages));
+      const uint32_t desc_lo0 = (uint32_t)desc0, desc_hi = (uint32_t)(desc0 >> 32);
+      const uint32_t stage_step = (uint32_t)(stage_size >> 4);
+      uint32_t desc_lo = desc_lo0;
       Tile t;
       for (uint32_t li = 0; next_tile(t); li++) {
         const int acc = (int)(li & 1);
@@ -332,46 +327,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t d = tmem_base + (uint32_t)(acc * kFp8MaxWidth);
         const uint32_t idesc0 = idesc_mxf8(256, t.width, 0);
         bool ok = true;
-        for (int kc = 0; kc < a.kchunks; kc++) {
-          const int sub = kc & 3;
-          const uint32_t scales = tmem_base + kScaleBase + (uint32_t)(slot * kSlotCols);
-          if (sub == 0) {
-            if (!mbar_wait(&sfull[slot], sphase, a.timeout_ns, abort_flag)) {
-              ok = false;
-              give_up();
-              break;
-            }
-            tc_fence_after();
-            const uint64_t ds = scale_block_desc(smem_addr(slots + slot * kSlotBytes));
-            tmem_cp_scales_pair(scales, ds);
-            tmem_cp_scales_pair(scales + 4, ds + (512 >> 4));
-            if (t.width > 128) tmem_cp_scales_pair(scales + 8, ds + (1024 >> 4));
-          }
-          if (!mbar_wait(&full[stage], phase, a.timeout_ns, abort_flag)) {
+        for (int kc = 0; kc < a.kchunks && ok; kc += 4) {  // a scale slot's chunks
+          if (!mbar_wait(&sfull[slot], sphase, a.timeout_ns, abort_flag)) {
             ok = false;
-            give_up();
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_addr(stages + stage * stage_size);
-          const uint64_t da = sw128_kmajor_desc(sa), db = sw128_kmajor_desc(sa + kRowBytes);
-          const uint32_t idesc = idesc0 | ((uint32_t)sub << 4) | ((uint32_t)sub << 29);
+          const uint32_t scales = tmem_base + kScaleBase + (uint32_t)(slot * kSlotCols);
+          const uint64_t ds = scale_block_desc(smem_addr(slots) + (uint32_t)(slot * kSlotBytes));
+          tmem_cp_scales_pair(scales, ds);
+          tmem_cp_scales_pair(scales + 4, ds + (512 >> 4));
+          if (t.width > 128) tmem_cp_scales_pair(scales + 8, ds + (1024 >> 4));
 #pragma unroll
-          for (int kk = 0; kk < 4; kk++)
-            mma_mxf8_pair(d, da + 2ull * kk, db + 2ull * kk, idesc, scales, scales + 4, (kc | kk) != 0 ? 1u : 0u);
-          mma_commit_pair_mc(&empty[stage], (uint16_t)0x3);
-          if (++stage == n_stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          if (sub == 3 || kc + 1 == a.kchunks) {
-            mma_commit_pair_mc(&sempty[slot], (uint16_t)0x3);
-            if (++slot == kScaleSlots) {
-              slot = 0;
-              sphase ^= 1u;
+          for (int sub = 0; sub < 4; sub++) {
+            if (kc + sub >= a.kchunks) break;
+            if (!mbar_wait(&full[stage], phase, a.timeout_ns, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            mma_mxf8_pair_chunk(d, desc_lo, desc_lo + (kRowBytes >> 4), desc_hi, idesc0 | sub << 4 | (uint32_t)sub << 29,
+                                scales, scales + 4, (uint32_t)(kc + sub));
+            mma_commit_pair_mc(&empty[stage], (uint16_t)0x3);
+            desc_lo += stage_step;
+            if (++stage == n_stages) {
+              stage = 0;
+              phase ^= 1u;
+              desc_lo = desc_lo0;
             }
           }
+          mma_commit_pair_mc(&sempty[slot], (uint16_t)0x3);
+          if (++slot == kScaleSlots) {
+            slot = 0;
+            sphase ^= 1u;
+          }
         }
+        if (!ok) give_up();
         if (!ok) break;
         mma_commit_pair_mc(&tfull[acc], (uint16_t)0x3);
       }
@@ -387,7 +378,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     using T = typename Out<kType>::T;
     const int quarter = warp & 3;
     const int first = (warp >> 2 & 1) * 32;  // this warp's 32-query groups: every other one
-    const int half_rows = a.tile_rows >> 1;
     const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0), nempty0 = mapa_shared(smem_addr(&nempty[0]), 0);
     for (uint32_t li = 0;; li++) {
       Tile t;
@@ -396,9 +386,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!__all_sync(0xFFFFFFFFu, next_tile(t))) break;
       const int acc = (int)(li & 1);
       // this warp's rows of the tile
-      int rows = t.rows - (int)rank * half_rows;
-      rows = (rows < half_rows ? rows : half_rows) - quarter * 32;
-      T* o = (T*)a.out + (int64_t)(t.query + first) * a.ldo + t.col + (int)rank * half_rows + quarter * 32;
+      int rows = t.rows - (int)rank * t.half;
+      rows = (rows < t.half ? rows : t.half) - quarter * 32;
+      T* o = (T*)a.out + (int64_t)(t.query + first) * a.ldo + t.col + (int)rank * t.half + quarter * 32;
       const bool ok = !*abort_flag && mbar_wait(&tfull[acc], (li >> 1) & 1u, a.timeout_ns, abort_flag);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         if (lane == 0) give_up();
@@ -449,8 +439,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (part > 0) wait_for_prep();
     Tile t;
     while (__all_sync(0xFFFFFFFFu, next_tile(t))) {
-      const int64_t first = (part == 0 ? t.row + rank * (uint32_t)(a.tile_rows >> 1) : t.query + (uint32_t)(part - 1) * 128u) + lane;
-      const int count = part == 0 ? a.tile_rows >> 1 : t.width - (part - 1) * 128;
+      const int64_t first = (part == 0 ? t.row + rank * (uint32_t)t.half : t.query + (uint32_t)(part - 1) * 128u) + lane;
+      const int count = part == 0 ? t.half : t.width - (part - 1) * 128;
       const uint8_t* at[4];
       bool in[4];
 #pragma unroll
@@ -507,16 +497,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     Finder finder(a);
     const uint32_t at[2] = {mapa_shared(smem_addr(tile_slots), 0), mapa_shared(smem_addr(tile_slots), 1)};
     const uint32_t bar[2] = {mapa_shared(smem_addr(nfull), 0), mapa_shared(smem_addr(nfull), 1)};
+    // The cluster's first tile is known to every role.  With groups the number after the one in hand is on
+    // its way while the group is looked up.
+    unsigned long long taken = 0;
+    auto take = [&]() {
+      if (a.next_tile && lane == 0) taken = atomicAdd(a.next_tile, 1ull);
+    };
     int64_t p = unit;
-    bool own = grouped;  // the first number is the cluster's own, and without groups known to every role
-    for (int width = 1; width != 0; own = false) {
-      if (!own && a.next_tile) {
-        unsigned long long n = 0;
-        if (lane == 0) n = atomicAdd(a.next_tile, 1ull);
-        p = units + (int64_t)__shfl_sync(0xFFFFFFFFu, n, 0);
-      } else if (!own) {
-        p += units;
-      }
+    auto advance = [&]() {
+      if (!grouped) take();
+      p = a.next_tile ? units + (int64_t)__shfl_sync(0xFFFFFFFFu, taken, 0) : p + units;
+      if (grouped) take();
+    };
+    if (grouped) take();
+    advance();
+    for (int width = 1; width != 0; advance()) {
       const Tile t = finder.find(p);
       width = t.width;
       const bool ok = mbar_wait(&nempty[nslot], nphase ^ 1u, a.timeout_ns, abort_flag);
@@ -524,9 +519,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) give_up();
         break;
       }
-      uint64_t x, y;
-      pack_tile(t, x, y);
-      if (lane < 2) store_cluster_16(at[lane] + (uint32_t)nslot * 16u, bar[lane] + (uint32_t)nslot * 8u, x, y);
+      const ulonglong2 v = pack_tile(t);
+      if (lane < 2) store_cluster_16(at[lane] + (uint32_t)nslot * 16u, bar[lane] + (uint32_t)nslot * 8u, v.x, v.y);
       if (++nslot == a.tile_slots) {
         nslot = 0;
         nphase ^= 1u;
@@ -577,15 +571,23 @@ cudaError_t launch_typed(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, 
 
 Fp8Tiling fp8_tiling(int64_t nrows, int64_t nq, int64_t groups, int num_sms) {
   Fp8Tiling t{};
-  t.tile_rows = 256;
+  t.tile_rows = kFp8TileRows;
   t.query_tiles = (int)((nq + kFp8MaxWidth - 1) / kFp8MaxWidth);
-  if (groups > 0) {  // the widest tile any group can have
+  if (groups > 0) {  // the widest tile any group can have; its rows go by the group
     t.width = (int)(nq < kFp8MaxWidth ? (nq + 31) / 32 * 32 : kFp8MaxWidth);
     return t;
   }
   // equal tiles of at most kFp8MaxWidth queries
   t.width = (int)(((nq + t.query_tiles - 1) / t.query_tiles + 31) / 32 * 32);
   t.tiles = (nrows + t.tile_rows - 1) / t.tile_rows * t.query_tiles;
+  // Few queries and few tiles per cluster: the stored rows are what takes the time, so each cluster's
+  // turns get equal shares of them.
+  const int64_t units = num_sms / 2, turns = (t.tiles + units - 1) / units;
+  if (t.width <= 64 && turns > 1 && turns <= 8) {
+    const int64_t share = (nrows + turns * units - 1) / (turns * units);
+    t.tile_rows = (int)((share + 7) / 8 * 8);
+    t.tiles = (nrows + t.tile_rows - 1) / t.tile_rows;
+  }
   return t;
 }
 

@@ -297,14 +297,28 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, ui
 // scaling): scale_a / scale_b are TMEM addresses of scale columns -- row r's scale exponents are the
 // bytes of the 32-bit word at lane r % 32 of column r / 32, the same in all four lane quarters --
 // and the instruction descriptor names the byte.  Each CTA holds its own A rows' scales and every
-// B row's.
-__device__ __forceinline__ void mma_mxf8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+// B row's.  Here the four of a 128-byte K chunk (128-byte swizzle: K advances by 32 bytes, 2 in the
+// descriptors' address field), the first accumulating if `accumulate`; a_lo, b_lo and hi are the
+// halves of sw128_kmajor_desc.
+__device__ __forceinline__ void mma_mxf8_pair_chunk(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
+                                                    uint32_t idesc, uint32_t scale_a, uint32_t scale_b,
+                                                    uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(scale_a), "r"(scale_b)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %7, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %4, [%5], [%6], p;\n\t"
+      "add.s64 a, a, 2;\n\t"
+      "add.s64 b, b, 2;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %4, [%5], [%6], 1;\n\t"
+      "add.s64 a, a, 2;\n\t"
+      "add.s64 b, b, 2;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %4, [%5], [%6], 1;\n\t"
+      "add.s64 a, a, 2;\n\t"
+      "add.s64 b, b, 2;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %4, [%5], [%6], 1;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
       : "memory");
 }
 // Its instruction descriptor: e4m3 x e4m3, both K-major, E8M0 scales taken from byte `scale_id` of

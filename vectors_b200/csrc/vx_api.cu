@@ -2681,11 +2681,12 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
   const uint8_t *q_codes = (const uint8_t*)q.p, *q_scales = q.scales;
   const bool encode = q.type != VX_E4M3;
   const Fp8Tiling t = fp8_tiling(n, q.nq, row_off ? groups : 0, dev->sms);
-  // Tiles are taken from a counter where there are more than clusters (a product of groups may have any
-  // number), but not for 8 or fewer each if clearing it would need a launch: stored queries x 100k
-  // x 768 rows (5.3 tiles a cluster) 20.5 us in fixed turns, 21.9 with the counter; 2M rows 246 and 223.
-  const bool deal = row_off || t.tiles > (encode ? 1 : 8) * (int64_t)(dev->sms / 2);
-  const size_t off_bytes = row_off ? ((size_t)groups + 1) * sizeof(int64_t) : 0;
+  // Tiles are taken from a counter, but with 8 or fewer for each cluster in fixed turns: one query x
+  // 100k x 768 rows (5.8 tiles each) 18.5 us in turns, 19.9 with the counter; 2M rows 246 and 223.
+  const bool deal = row_off || t.tiles > 8 * (int64_t)(dev->sms / 2);
+  const int firsts = dev->sms / 2;
+  const size_t firsts_bytes = (size_t)firsts * 16, bounds_bytes = (size_t)groups * 16;
+  const size_t off_bytes = row_off ? firsts_bytes + bounds_bytes + ((size_t)groups + 1) * sizeof(int64_t) : 0;
   const size_t q_at = round_up(16 + off_bytes, 128);
   const size_t q_bytes = encode ? (size_t)q.nq * (pitch + scale_pitch) : 0;
   const bool prep = encode || deal;
@@ -2698,7 +2699,11 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
     uint8_t* buf = S.alloc<uint8_t>(q_at + q_bytes);
     Fp8WriteArgs w{};
     if (deal) a.next_tile = (unsigned long long*)buf;
-    if (row_off) a.groups = Fp8Groups{row_off, query_off, groups, n, q.nq, max_cols, t.tile_rows, (int64_t*)(buf + 16)};
+    if (row_off) {
+      uint8_t* at = buf + 16;
+      a.groups = Fp8Groups{row_off, query_off, groups, n, q.nq, max_cols, (int4*)(at + firsts_bytes),
+                           (int64_t*)(at + firsts_bytes + bounds_bytes), (ulonglong2*)at, firsts};
+    }
     if (encode) {
       w.rows = q.p;
       w.type = q.type;
@@ -2714,11 +2719,15 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
     VX_LAUNCH(1, launch_fp8_prepare(w, a.groups, a.next_tile, st));
   }
   Fp8Maps maps{};
-  fp8_map(&maps.rows, codes, n, pitch, t.tile_rows / 2);
-  if (!row_off)
+  if (!row_off) {
+    fp8_map(&maps.rows[0], codes, n, pitch, t.tile_rows / 2);
     fp8_map(&maps.queries[0], q_codes, q.nq, pitch, t.width / 2);
-  else
-    for (int i = 0; i < 3; i++) fp8_map(&maps.queries[i], q_codes, q.nq, pitch, 64 >> i);
+  } else {
+    for (int i = 0; i < 4; i++) {
+      fp8_map(&maps.rows[i], codes, n, pitch, 128 >> i);
+      fp8_map(&maps.queries[i], q_codes, q.nq, pitch, 128 >> i);
+    }
+  }
   a.row_scales = scales;
   a.nrows = n;
   a.query_scales = q_scales;
