@@ -107,10 +107,11 @@ __device__ __forceinline__ int scale_byte(uint32_t amax_bits) {
 
 // ---------------------------------------------------------------- repeated slots
 // Where several rows of a batch name one slot, the last of them is kept.  Up to kFp8DirectSlots
-// rows: each row looks for its slot among the later rows.  Above: owner[slot] becomes the largest
-// row index that names the slot, without clearing `owner` first: every row stores its index (some
-// row's index is left), then every row raises the entry to its own.  The three launches overlap:
-// each begins before the one before it ends and waits for it where it needs its results.
+// rows: the lanes of a block look for its slot among the later rows.  Above: owner[slot] becomes the
+// largest row index that names the slot, without clearing `owner` first: every row stores its index
+// (some row's index is left), then every row raises the entry to its own.  The three launches overlap:
+// each begins before the one before it ends and waits for it where it needs its results.  (One CTA for
+// both steps takes 13 us for 10k scattered slots, the two launches 2.)
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -167,12 +168,12 @@ __global__ void __launch_bounds__(kThreads, 6) fp8_write_kernel(const Fp8WriteAr
     }
     if (a.owner && first) wait_for_launch_before();
     bool keep = slot >= 0;
-    if (keep && a.slots) {
-      if (a.owner) {
-        keep = __ldcg(a.owner + slot) == (int32_t)row;
-      } else {
-        for (int64_t j = row + 1; j < a.n; j++) keep &= slot_at(a.slots, a.slot_bytes, j) != slot;
-      }
+    if (a.owner) {
+      if (keep) keep = __ldcg(a.owner + slot) == (int32_t)row;
+    } else if (a.slots) {
+      if (keep)
+        for (int j = (int)row + 1 + part; j < (int)a.n; j += 8) keep &= slot_at(a.slots, a.slot_bytes, j) != slot;
+      keep = (__ballot_sync(0xFFFFFFFFu, !keep) >> (threadIdx.x & 24) & 0xFFu) == 0;
     }
     uint32_t m = keep ? largest<T>(r) : 0u;
 #pragma unroll

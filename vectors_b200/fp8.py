@@ -132,28 +132,20 @@ def _slots(slots, device: int):
     return slots.contiguous()
 
 
-def _queued(f):
-    """Runs a function with its ``stream`` argument made current, so that what it allocates or copies
-    belongs to that stream."""
-
-    @functools.wraps(f)
-    def call(*args, stream=None, **more):
-        if stream is None:
-            return f(*args, **more)
-        at = next((t for t in (*args, *more.values()) if isinstance(t, torch.Tensor) and t.is_cuda), None)
-        device = at.get_device() if at is not None else torch.cuda.current_device()
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
-            return f(*args, **more)
-
-    return call
+def _on_stream(stream: int, codes):
+    """Makes a raw stream current, so that what a call allocates or copies belongs to it."""
+    device = codes.get_device() if isinstance(codes, torch.Tensor) and codes.is_cuda else None
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
-@_queued
-def fp8_write_device(rows, codes, scales, slots=None, first: int = 0) -> None:
+def fp8_write_device(rows, codes, scales, slots=None, first: int = 0, stream=None) -> None:
     """Quantises rows [n][dim] (float32 / float16 / bfloat16) into a store: row i into slot
     ``slots[i]`` (int32 or int64; outside [0, capacity) the row is skipped; of rows that name the same
     slot the last is kept), or into ``first + i`` without slots.  Other rows stay as they are.  Writes
     that overlap on other streams are ordered by the caller."""
+    if stream is not None:
+        with _on_stream(stream, codes):
+            return fp8_write_device(rows, codes, scales, slots, first)
     capacity, kp, device = _store(codes, scales)
     rows, n, dim, step = _matrix(rows, device, "rows")
     if dim > kp or dim <= kp - BLOCK:
@@ -168,12 +160,14 @@ def fp8_write_device(rows, codes, scales, slots=None, first: int = 0) -> None:
                                         codes.data_ptr(), scales.data_ptr(), capacity, _raw_stream(device)))
 
 
-@_queued
 def fp8_read_device(codes, scales, dim: int, slots=None, first: int = 0, count: Optional[int] = None, dtype=None,
-                    out=None):
+                    out=None, stream=None):
     """Stored rows as floats [n][dim] (``dtype`` float32, float16 or bfloat16): those of ``slots``
     (int32 or int64, of any search result; outside [0, capacity) a row of zeros), or ``count`` rows
     from ``first`` (default: to the end)."""
+    if stream is not None:
+        with _on_stream(stream, codes):
+            return fp8_read_device(codes, scales, dim, slots, first, count, dtype, out)
     capacity, kp, device = _store(codes, scales)
     if dim > kp or dim <= kp - BLOCK:
         raise IllegalArgumentException(f"dimension {dim} does not match the store's {kp} columns")
@@ -204,11 +198,13 @@ def _queries(queries, query_scales, kp: int, device: int):
     return queries, nq, dim, _type_of(queries, "queries"), None, step
 
 
-@_queued
-def fp8_scores_device(queries, codes, scales, query_scales=None, dtype=None, out=None):
+def fp8_scores_device(queries, codes, scales, query_scales=None, dtype=None, out=None, stream=None):
     """dot(query, row) of every query and stored row: [nq][rows] of ``dtype`` (float32, float16 or
     bfloat16), into ``out`` if given.  Queries are floats [nq][dim], quantised as stored rows are, or
     stored rows themselves (codes, with their ``query_scales``)."""
+    if stream is not None:
+        with _on_stream(stream, codes):
+            return fp8_scores_device(queries, codes, scales, query_scales, dtype, out)
     n, kp, device = _store(codes, scales)
     q, nq, dim, kind, qs, step = _queries(queries, query_scales, kp, device)
     if nq == 0:
@@ -228,14 +224,17 @@ def _offsets(t, device: int, name: str) -> int:
     return t.shape[0] - 1
 
 
-@_queued
 def fp8_scores_grouped_device(queries, query_offsets, codes, scales, row_offsets, query_scales=None,
-                              max_rows: Optional[int] = None, dtype=None, out=None):
+                              max_rows: Optional[int] = None, dtype=None, out=None, stream=None):
     """For each group g the products of queries ``query_offsets[g]:query_offsets[g + 1]`` with stored rows
     ``row_offsets[g]:row_offsets[g + 1]`` (int64 CUDA tensors [groups + 1]; sizes may differ or be zero):
     out[i][j] for the group's j-th row, [nq][max_rows].  Without ``out`` the result is new and zero
     past each group's rows; in a given ``out`` (whose width is max_rows) those values, and rows of
     queries in no group, stay as they are.  A group's rows past max_rows are not scored."""
+    if stream is not None:
+        with _on_stream(stream, codes):
+            return fp8_scores_grouped_device(queries, query_offsets, codes, scales, row_offsets, query_scales, max_rows,
+                                             dtype, out)
     n, kp, device = _store(codes, scales)
     q, nq, dim, kind, qs, step = _queries(queries, query_scales, kp, device)
     groups = _offsets(query_offsets, device, "query_offsets")
