@@ -381,7 +381,8 @@ VX_API int vx_fp8_read_device(int32_t device, const uint8_t* codes, const uint8_
  * out_stride elements apart, out_type VX_F32 / VX_F16 / VX_BF16.  Queries [nq][dim] of VX_F32 / VX_F16 /
  * VX_BF16, query_stride elements apart, are quantised as vx_fp8_write_device does; or they are stored
  * rows: query_type VX_E4M3 with their codes and query_scales (query_stride is not used).  Products are
- * exact and summed in fp32; a NaN block makes its query's or row's results NaN. */
+ * exact and summed in fp32 (a result whose partial sums leave fp32's range is not finite); a NaN block
+ * makes its query's or row's results NaN. */
 VX_API int vx_fp8_scores_device(int32_t device, const void* queries, int32_t query_type, const uint8_t* query_scales,
                                 int64_t nq, int64_t query_stride, const uint8_t* codes, const uint8_t* scales,
                                 int64_t n, int32_t dim, void* out, int32_t out_type, int64_t out_stride, void* stream);
@@ -391,7 +392,8 @@ VX_API int vx_fp8_scores_device(int32_t device, const void* queries, int32_t que
  * out[i][j - row_offsets[g]] for query i of group g, out [nq][max_rows] out_stride elements apart; results
  * past a group's rows, and rows of out in no group, are left as they are; a group's rows past max_rows are
  * not scored.  Offsets are clamped to the operands' sizes and an end below its start is an empty
- * group, so no offsets read or write out of range; groups whose queries overlap write the same results. */
+ * group, so no offsets read or write out of range.  Groups may share rows; a query that several groups
+ * name gets one of their results in each place. */
 VX_API int vx_fp8_scores_grouped_device(int32_t device, const void* queries, int32_t query_type,
                                         const uint8_t* query_scales, int64_t nq, int64_t query_stride,
                                         const int64_t* query_offsets, const uint8_t* codes, const uint8_t* scales,

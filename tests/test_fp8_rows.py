@@ -561,6 +561,100 @@ def test_refusals_of_tensors():
             call()
 
 
+@pytest.mark.gpu
+def test_scores_of_extreme_scales():
+    """Scales whose product is ordinary, leaves fp32 upwards (infinity) or downwards (at most its smallest
+    normal number off)."""
+    import torch
+
+    q, x = rows_of(40, 256, 1, 0.5).astype(np.float64), rows_of(300, 256, 2, 0.5).astype(np.float64)
+    with np.errstate(over="ignore"):
+        for eq, er in ((100, -100), (-110, 110), (-60, -70), (-100, -100), (70, 70)):
+            a, b = (q * 2.0 ** eq).astype(np.float32), (x * 2.0 ** er).astype(np.float32)
+            codes, scales = _store(b)
+            got = vx.fp8_scores_device(torch.from_numpy(a).cuda(), codes, scales).cpu().numpy().astype(np.float64)
+            dq, dr = decode(*encode(a)), decode(_bytes(codes), scales.cpu().numpy())
+            want, tol = dq @ dr.T, bound(dq, dr, "float32") + 2.0 ** -126
+            # where single terms pass fp32's range (2^140 here), a partial sum is infinite before the last term
+            # is in, with that partial sum's sign and not the result's: only "not finite" follows
+            huge = np.abs(want) > 2.0 ** 129
+            assert not np.isfinite(got[huge]).any()
+            fine = np.abs(want) + tol < 2.0 ** 127
+            assert (np.abs(got - want) <= tol)[fine].all()
+            assert fine.all() or eq + er > 100
+
+
+@pytest.mark.gpu
+def test_groups_that_share_rows():
+    """The same rows scored for several groups, and a group with the same offsets twice."""
+    import torch
+
+    q, x = rows_of(50, 200, 1), rows_of(900, 200, 2)
+    codes, scales = _store(x)
+    dq, dr = decode(*encode(q)), decode(_bytes(codes), scales.cpu().numpy())
+    want = dq @ dr.T
+    tol = bound(dq, dr, "float32")
+    # 10 queries x rows 0-600, none, 20 x none (descending), 20 x 300-900: offsets ascend only per operand's rule
+    qo = torch.tensor([0, 10, 10, 30, 50], device="cuda")
+    ro = torch.tensor([0, 600, 600, 300, 900], device="cuda")
+    out = torch.full((50, 600), -1.0, device="cuda")
+    vx.fp8_scores_grouped_device(torch.from_numpy(q).cuda(), qo, codes, scales, ro, out=out)
+    got = out.cpu().numpy().astype(np.float64)
+    assert (np.abs(got[:10] - want[:10, :600]) <= tol[:10, :600]).all()
+    assert (got[10:30] == -1).all()
+    assert (np.abs(got[30:] - want[30:, 300:900]) <= tol[30:, 300:900]).all()
+
+
+@pytest.mark.gpu
+def test_store_past_32_bits():
+    """Slots whose codes lie past 2^32 bytes, written, read back and scored."""
+    import torch
+
+    if torch.cuda.get_device_properties(0).total_memory < 32 << 30:
+        pytest.skip("needs 32 GB")
+    capacity, dim = 4_400_000, 1000
+    codes, scales = vx.fp8_empty(capacity, dim)
+    x = rows_of(700, dim, 1)
+    slots = torch.cat([torch.arange(capacity - 600, capacity), torch.arange(100)]).cuda()
+    vx.fp8_write_device(torch.from_numpy(x).cuda(), codes, scales, slots=slots)
+    c, s = encode(x)
+    assert np.array_equal(_bytes(codes[-600:]), c[:600]) and np.array_equal(scales[-600:].cpu().numpy(), s[:600])
+    back = vx.fp8_read_device(codes, scales, dim, slots=slots)
+    assert np.array_equal(back.cpu().numpy(), decode(c, s)[:, :dim].astype(np.float32))
+    assert torch.equal(vx.fp8_read_device(codes, scales, dim, first=capacity - 600), back[:600])
+    q = rows_of(3, dim, 2)
+    got = vx.fp8_scores_device(torch.from_numpy(q).cuda(), codes, scales)
+    dq, dr = decode(*encode(q)), decode(c, s)
+    assert (np.abs(got[:, slots].cpu().numpy() - dq @ dr.T) <= bound(dq, dr, "float32")).all()
+    assert not got[:, 100:-600].any()
+    ro = torch.tensor([0, 100, capacity - 600, capacity], device="cuda")
+    out = torch.zeros(3, 600, device="cuda")
+    vx.fp8_scores_grouped_device(torch.from_numpy(q).cuda(), torch.tensor([0, 1, 1, 3], device="cuda"), codes, scales, ro,
+                                 out=out)
+    assert torch.equal(out[0, :100], got[0, :100]) and torch.equal(out[1:], got[1:, -600:])
+
+
+@pytest.mark.gpu
+def test_results_past_32_bits():
+    """A score matrix of more than 2^31 results."""
+    import torch
+
+    if torch.cuda.get_device_properties(0).total_memory < 32 << 30:
+        pytest.skip("needs 32 GB")
+    q, x = rows_of(47000, 128, 1, 1.0), rows_of(46000, 128, 2, 1.0)
+    qc, qs, codes, scales = *vx.fp8_empty(47000, 128), *vx.fp8_empty(46000, 128)
+    vx.fp8_write_device(torch.from_numpy(q).cuda(), qc, qs)
+    vx.fp8_write_device(torch.from_numpy(x).cuda(), codes, scales)
+    got = vx.fp8_scores_device(qc, codes, scales, query_scales=qs, dtype=torch.bfloat16)
+    assert got.numel() > 2 ** 31
+    for at in (slice(0, 50), slice(23400, 23450), slice(46950, 47000)):
+        part = vx.fp8_scores_device(qc[at], codes, scales, query_scales=qs[at], dtype=torch.bfloat16)
+        assert torch.equal(got[at], part)
+    at = slice(46990, 47000)
+    dq, dr = decode(_bytes(qc[at]), qs[at].cpu().numpy()), decode(_bytes(codes), scales.cpu().numpy())
+    assert (np.abs(got[at].float().cpu().numpy() - dq @ dr.T) <= bound(dq, dr, "bfloat16")).all()
+
+
 # ---------------------------------------------------------------- streams, graphs, the operators together
 @pytest.mark.gpu
 def test_other_stream_and_graph():
