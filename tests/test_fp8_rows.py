@@ -378,7 +378,7 @@ def test_every_code_and_scale_reads_back():
 @pytest.mark.gpu
 @pytest.mark.parametrize("nq, n, dim", [(1, 1, 1), (1, 255, 100), (16, 256, 128), (17, 257, 129), (31, 300, 512), (33, 1000, 513),
                                         (224, 513, 640), (225, 700, 768), (100, 40000, 64), (500, 1111, 1500), (3, 70000, 200),
-                                        (1000, 300, 2048)])
+                                        (1000, 300, 2048), (64, 20000, 256), (37, 5003, 300), (1, 600, 16384)])
 @pytest.mark.parametrize("out", ["float32", "float16", "bfloat16"])
 def test_scores(nq, n, dim, out):
     import torch

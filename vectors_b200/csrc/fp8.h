@@ -97,8 +97,14 @@ struct Fp8ScoreArgs {
   int query_tiles;    // without groups
   int width;          // queries of the widest tile, a multiple of 32
   int tile_rows;      // stored rows of a tile
+  // A few float queries that every cluster quantises for itself (resident queries): type a vx_dtype
+  const void* queries;  // null: query_scales and the tensor maps tell of stored rows
+  int query_type;
+  int dim;
+  int64_t query_stride;
   // filled in by launch_fp8_scores
   int stages;
+  int stage_bytes;
   int tile_slots;
   int wait_first;
 };
@@ -115,6 +121,9 @@ struct Fp8Tiling {
   int width, tile_rows, query_tiles;
   int64_t tiles;
 };
+// Whether a product's float queries are quantised inside it: few of them, and blocks for one round of
+// its epilogue warps.
+bool fp8_resident(int64_t nq, int dim, const Fp8Tiling& t);
 Fp8Tiling fp8_tiling(int64_t nrows, int64_t nq, int64_t groups, int num_sms);
 // after_prep: the launch before this one on `st` is launch_fp8_prepare's; this one may begin before it
 // ends.

@@ -9,16 +9,17 @@
 // sum would have to be read from TMEM and multiplied in the FP32 pipe, which takes as long as the
 // MMAs themselves.)
 //
-// Tiling.  2-CTA clusters (cta_group::2), 256 stored rows x up to 224 queries.  The stored rows are
-// the MMA's M operand, so a TMEM lane holds one stored row and an epilogue warp has 32 consecutive
+// Tiling.  2-CTA clusters (cta_group::2), up to 256 stored rows x up to 224 queries.  The stored rows
+// are the MMA's M operand, so a TMEM lane holds one stored row and an epilogue warp has 32 consecutive
 // results of each query, which it stores as they are: 32 lanes, 4 (or 2) bytes each.  (16 bytes a
 // lane, brought together by shuffles or through shared memory, or TMA stores from there, were
 // slower: 400 MB of fp32 results 115, 90 and 89 us against 85; 200 MB of bf16 84, 68 and 91 against
-// 50.)  The queries are
-// its N operand, any multiple of 32, so few queries cost few MMA cycles and the kernel then streams
-// the stored rows at HBM speed; each CTA stages its 128 rows and half the queries of a 128-byte K
-// chunk by TMA (128-byte swizzle).  224 and not 256 queries: two accumulators take 448 of the 512
-// TMEM columns and leave 60 for a ring of five scale slots.
+// 50.)  The queries are its N operand, any multiple of 32, so few queries cost few MMA cycles and the
+// kernel then streams the stored rows at HBM speed (one query x 2M x 768: 7.0 TB/s); each CTA stages
+// its half of the rows and of the queries of a 128-byte K chunk by TMA (128-byte swizzle).  224 and
+// not 256 queries: two accumulators take 448 of the 512 TMEM columns and leave 60 for a ring of five
+// scale slots.  At 8192 x 65536 x 1024 with bf16 results the tensor pipe is busy 81 % of a lone call
+// (434 us, 2.5 PFLOP/s); back to back the card's power limit holds it to 2.0.
 //
 // Scales.  A slot holds the scale words of four K chunks (512 dimensions): 128 words for the CTA's
 // rows and up to 256 for the queries.  A stored row's scale bytes are consecutive, so a 32-bit load
@@ -28,15 +29,20 @@
 // its MMAs.  (Stored from registers with tcgen05.st, or handed over with a release at cluster scope,
 // a slot took 1,400-2,000 cycles, more than its MMAs.)
 //
-// Tiles.  Clusters take tiles from a counter, not in fixed turns: with large results the SMs' shares
-// of the write bandwidth differ by half (the slowest unit of 1000 x 100k fp32 results took 87 us
-// with the median at 67).  One warp of the leader finds the next tile, with groups by a search over
-// 32 places at once, and sends its description to every role of both CTAs.
+// Tiles.  Clusters take tiles from a counter where there are many: with large results the SMs' shares of
+// the write bandwidth differ (the slowest unit of 1000 x 100k x 128 in fixed turns took 87 us with the
+// median at 67).  One warp of the leader finds the next tile, with groups by looking at 128 groups'
+// offsets at once, and sends its description to every role of both CTAs; a cluster's first tile waits
+// for nobody.
+//
+// Few float queries.  Up to 64 queries of 128 blocks in all are quantised by each cluster for itself, into
+// shared memory in the MMA's layout, where they stay for all its tiles: one launch and no scratch
+// (one query x 10k x 768: 10.8 -> 8.2 us a call; x 100k: 20.7 -> 18.5; 37 x 5,003 x 300: 10.8 -> 10.2).
 //
 // Warps: 0 rows by TMA, 1 TMEM and (leader CTA) MMA, 2 row scales, 3-4 query scales, 5 hand-over of
-// scales, 6 queries by TMA, 7 (leader CTA) tiles, 8-15 epilogue (two per TMEM lane quarter, taking 32-query groups in
-// turn).  Every wait is bounded; on expiry the error word is set, the roles unwind and
-// TMEM is released.
+// scales, 6 queries by TMA, 7 (leader CTA) tiles, 8-15 epilogue (two per TMEM lane quarter, taking
+// 32-query groups in turn).  Every wait is bounded; on expiry the error word is set, the roles unwind
+// and TMEM is released.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -44,6 +50,7 @@
 
 #include "../../include/vx.h"
 #include "fp8.h"
+#include "fp8_encode.cuh"
 #include "fp8_groups.cuh"
 #include "sm100.cuh"
 
@@ -60,11 +67,12 @@ constexpr int kSlotCols = 12;
 constexpr int kSlotBytes = 1536;  // 128 row words, then up to 256 query words
 constexpr uint32_t kScaleBase = 2 * kFp8MaxWidth;
 constexpr size_t kMaxSmem = 232448;
+constexpr int kMaxResident = 64 << 10;  // bytes of a CTA's resident queries
 constexpr size_t kTailBytes = kScaleSlots * kSlotBytes + 1024;  // scale slots, barriers, tiles
 constexpr int kMaxStages = 12;
 constexpr int kTileSlots = 8;  // most tiles on their way
 
-static_assert(2 * kMaxStages + 3 * kScaleSlots + 4 + 2 * kTileSlots + 1 <= 64, "barriers");
+static_assert(2 * kMaxStages + 3 * kScaleSlots + 4 + 2 * kTileSlots + 2 <= 64, "barriers");
 static_assert(kScaleBase + kScaleSlots * kSlotCols <= kTmemCols, "TMEM columns");
 
 __host__ __device__ constexpr size_t stage_bytes(int width) { return kRowBytes + (size_t)width / 2 * 128; }
@@ -151,14 +159,68 @@ struct Out<VX_BF16> {
   static __device__ __forceinline__ T of(uint32_t v) { return __float2bfloat16_rn(__uint_as_float(v)); }
 };
 
-template <int kType>
+// Shared memory of resident queries: this CTA's half of the codes, chunk by chunk with 128-byte swizzle,
+// and every query's scale words as scale slots have them.
+__host__ __device__ __forceinline__ uint32_t resident_codes(const Fp8ScoreArgs& a) {
+  return (uint32_t)(a.width / 2 * 128 * a.kchunks);
+}
+__host__ __device__ __forceinline__ uint32_t resident_words(const Fp8ScoreArgs& a) {
+  return (uint32_t)((a.kchunks + 3) / 4 * 512);
+}
+
+// Quantises the queries, by the eight epilogue warps: every query's scales and this CTA's half of the
+// codes.  Places past the last query keep what they hold: they reach only columns that are not stored.
+template <class T>
+__device__ __forceinline__ void encode_resident(const Fp8ScoreArgs& a, uint8_t* codes, uint8_t* words, uint32_t rank) {
+  constexpr int kWords = (int)sizeof(T);  // of a piece of 4
+  const int part = threadIdx.x & 7, group = ((int)threadIdx.x - 256) >> 3;
+  const int blocks = (int)a.nq * a.kchunks, half = a.width >> 1;
+  const bool vec = ((uintptr_t)a.queries | (uintptr_t)(a.query_stride * (int64_t)sizeof(T))) % (4 * sizeof(T)) == 0;
+  uint32_t r[4][4 * kWords];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {  // at most 128 blocks: all on their way at once
+    const int block = j * 32 + group;
+    if (block >= blocks) continue;
+    const int q = block / a.kchunks, k = block % a.kchunks * kFp8Block;
+    const T* x = (const T*)a.queries + q * a.query_stride;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int at = k + (i * 8 + part) * 4;
+      if (vec) load_piece<T, 4, true>(x, at, a.dim, r[j] + i * kWords);
+      else load_piece<T, 4, false>(x, at, a.dim, r[j] + i * kWords);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int block = j * 32 + group;
+    uint32_t m = block < blocks ? largest<T>(r[j]) : 0u;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (block >= blocks) continue;
+    const int q = block / a.kchunks, kc = block % a.kchunks;
+    const int b = scale_byte(m);
+    if (part == 0) words[kc / 4 * 512 + (q & 31) * 16 + (q >> 5) * 4 + (kc & 3)] = (uint8_t)b;
+    const int row = q - (int)rank * half;
+    if (row < 0 || row >= half) continue;
+    uint8_t* to = codes + (kc * half + row) * 128;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int at = (i * 8 + part) * 4;
+      *(uint32_t*)(to + (((at >> 4) ^ (row & 7)) << 4 | (at & 15))) = four_codes<T>(r[j] + i * kWords, 0, b);
+    }
+  }
+}
+
+template <int kType, bool kResident>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_scores_kernel(const __grid_constant__ Fp8Maps maps, const __grid_constant__ Fp8ScoreArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int n_stages = a.stages;
-  const size_t stage_size = stage_bytes(a.width);
-  uint8_t* slots = stages + n_stages * stage_size;
+  const uint32_t stage_size = (uint32_t)a.stage_bytes;
+  uint8_t* resident = stages + n_stages * stage_size;  // queries quantised here: codes, then scale words
+  uint8_t* resident_scales = resident + (kResident ? resident_codes(a) : 0);
+  uint8_t* slots = resident_scales + (kResident ? resident_words(a) : 0);
   uint64_t* full = (uint64_t*)(slots + kScaleSlots * kSlotBytes);
   uint64_t* empty = full + kMaxStages;
   uint64_t* landed = empty + kMaxStages;
@@ -169,6 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* nfull = tempty + 2;
   uint64_t* nempty = nfull + kTileSlots;
   uint64_t* drained = nempty + kTileSlots;
+  uint64_t* encoded = drained + 1;
   uint64_t* tile_slots = full + 64;  // 16-byte aligned
   uint32_t* tmem_slot = (uint32_t*)(tile_slots + 2 * kTileSlots);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
@@ -177,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
-  if (warp == 0 && lane < 2) prefetch_tmap(lane == 0 ? &maps.rows[0] : &maps.queries[0]);
+  if (warp == 0 && lane < 2 && (lane == 0 || !kResident)) prefetch_tmap(lane == 0 ? &maps.rows[0] : &maps.queries[0]);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stages; s++) {
@@ -185,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kScaleSlots; s++) {
-      mbar_init(&landed[s], 96);  // the lanes of the three loading warps
+      mbar_init(&landed[s], kResident ? 32 : 96);  // the lanes of the loading warps
       mbar_init(&sfull[s], 2);    // each CTA's hand-over
       mbar_init(&sempty[s], 1);
     }
@@ -198,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&nempty[s], 16);  // a stored tile has been read by every role before: the epilogue warps
     }
     mbar_init(drained, 1);
+    mbar_init(encoded, 16);  // the epilogue warps of both CTAs
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -260,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0 || warp == 6) {
     // ---------------- TMA: warp 0 the stored rows, warp 6 the queries
-    if (elect_one()) {
+    if ((warp == 0 || !kResident) && elect_one()) {
       const bool rows = warp == 0;
       const CUtensorMap* map = rows ? maps.rows : maps.queries;
       // query tiles are read again for every row tile
@@ -280,7 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           uint8_t* s = stages + stage * stage_size + (rows ? 0 : kRowBytes);
           const uint32_t bar = full0 + (uint32_t)(stage * 8);
-          if (rows && leader) mbar_arrive_expect_tx(&full[stage], 2u * 128u * (uint32_t)(count + (t.width >> 1)));
+          if (rows && leader)
+            mbar_arrive_expect_tx(&full[stage], 2u * 128u * (uint32_t)(count + (kResident ? 0 : t.width >> 1)));
           if (!grouped) {
             tma_load_2d_pair(s, map, bar, kc * 128, y0, policy);
           } else {
@@ -314,8 +379,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0, sphase = 0;
       const uint64_t desc0 = sw128_kmajor_desc(smem_addr(stages));
       const uint32_t desc_lo0 = (uint32_t)desc0, desc_hi = (uint32_t)(desc0 >> 32);
-      const uint32_t stage_step = (uint32_t)(stage_size >> 4);
+      const uint32_t stage_step = stage_size >> 4;
       uint32_t desc_lo = desc_lo0;
+      // the queries' operand: behind the rows' in each stage, or resident
+      const uint32_t resident_lo = (uint32_t)sw128_kmajor_desc(smem_addr(resident));
+      const uint32_t resident_step = (uint32_t)(a.width / 2 * 128) >> 4;
+      const uint64_t resident_ds = scale_block_desc(smem_addr(resident_scales));
+      if (kResident && !mbar_wait(encoded, 0, a.timeout_ns, abort_flag)) give_up();
       Tile t;
       for (uint32_t li = 0; next_tile(t); li++) {
         const int acc = (int)(li & 1);
@@ -336,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t scales = tmem_base + kScaleBase + (uint32_t)(slot * kSlotCols);
           const uint64_t ds = scale_block_desc(smem_addr(slots) + (uint32_t)(slot * kSlotBytes));
           tmem_cp_scales_pair(scales, ds);
-          tmem_cp_scales_pair(scales + 4, ds + (512 >> 4));
+          tmem_cp_scales_pair(scales + 4, kResident ? resident_ds + (uint64_t)(kc * (512 / 4) >> 4) : ds + (512 >> 4));
           if (t.width > 128) tmem_cp_scales_pair(scales + 8, ds + (1024 >> 4));
 #pragma unroll
           for (int sub = 0; sub < 4; sub++) {
@@ -346,7 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               break;
             }
             tc_fence_after();
-            mma_mxf8_pair_chunk(d, desc_lo, desc_lo + (kRowBytes >> 4), desc_hi, idesc0 | sub << 4 | (uint32_t)sub << 29,
+            const uint32_t b_lo = kResident ? resident_lo + (uint32_t)(kc + sub) * resident_step : desc_lo + (kRowBytes >> 4);
+            mma_mxf8_pair_chunk(d, desc_lo, b_lo, desc_hi, idesc0 | sub << 4 | (uint32_t)sub << 29,
                                 scales, scales + 4, (uint32_t)(kc + sub));
             mma_commit_pair_mc(&empty[stage], (uint16_t)0x3);
             desc_lo += stage_step;
@@ -379,6 +450,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;
     const int first = (warp >> 2 & 1) * 32;  // this warp's 32-query groups: every other one
     const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0), nempty0 = mapa_shared(smem_addr(&nempty[0]), 0);
+    if constexpr (kResident) {
+      if (a.query_type == VX_F32) encode_resident<float>(a, resident, resident_scales, rank);
+      else if (a.query_type == VX_F16) encode_resident<__half>(a, resident, resident_scales, rank);
+      else encode_resident<__nv_bfloat16>(a, resident, resident_scales, rank);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_pair(mapa_shared(smem_addr(encoded), 0));
+    }
     for (uint32_t li = 0;; li++) {
       Tile t;
       const bool sent = !first_tile;  // by the tile warp, in slot nslot
@@ -438,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t sphase = 0;
     if (part > 0) wait_for_prep();
     Tile t;
-    while (__all_sync(0xFFFFFFFFu, next_tile(t))) {
+    while ((part == 0 || !kResident) && __all_sync(0xFFFFFFFFu, next_tile(t))) {
       const int64_t first = (part == 0 ? t.row + rank * (uint32_t)t.half : t.query + (uint32_t)(part - 1) * 128u) + lane;
       const int count = part == 0 ? t.half : t.width - (part - 1) * 128;
       const uint8_t* at[4];
@@ -537,10 +616,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int kType>
+template <int kType, bool kResident>
 cudaError_t launch_typed(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, size_t smem, bool after_prep,
                          cudaStream_t st) {
-  auto kern = fp8_scores_kernel<kType>;
+  auto kern = fp8_scores_kernel<kType, kResident>;
   static std::atomic<uint64_t> sized{0};  // bit d: done for device d
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
@@ -567,6 +646,13 @@ cudaError_t launch_typed(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, 
   return cudaLaunchKernelEx(&cfg, kern, maps, a);
 }
 
+template <int kType>
+cudaError_t launch_out(const Fp8Maps& maps, const Fp8ScoreArgs& a, int units, size_t smem, bool after_prep,
+                       cudaStream_t st) {
+  return a.queries ? launch_typed<kType, true>(maps, a, units, smem, after_prep, st)
+                   : launch_typed<kType, false>(maps, a, units, smem, after_prep, st);
+}
+
 }  // namespace
 
 Fp8Tiling fp8_tiling(int64_t nrows, int64_t nq, int64_t groups, int num_sms) {
@@ -591,24 +677,32 @@ Fp8Tiling fp8_tiling(int64_t nrows, int64_t nq, int64_t groups, int num_sms) {
   return t;
 }
 
+bool fp8_resident(int64_t nq, int dim, const Fp8Tiling& t) {
+  return t.query_tiles == 1 && t.width <= 64 && nq * fp8_blocks(dim) <= 128 &&
+         t.width / 2 * fp8_code_pitch(dim) <= kMaxResident;
+}
+
 cudaError_t launch_fp8_scores(const Fp8Maps& maps, const Fp8ScoreArgs& args, int out_type, int num_sms, bool after_prep,
                               cudaStream_t st) {
   Fp8ScoreArgs a = args;
   int64_t units = num_sms / 2;
   if (!a.groups.row_off && units > a.tiles) units = a.tiles;
   if (units < 1) units = 1;
-  a.stages = (int)((kMaxSmem - 1024 - kTailBytes) / stage_bytes(a.width));
+  const size_t tail = kTailBytes + (a.queries ? resident_codes(a) + resident_words(a) : 0);
+  a.stage_bytes = (int)(a.queries ? kRowBytes : stage_bytes(a.width));
+  a.stages = (int)((kMaxSmem - 1024 - tail) / a.stage_bytes);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
+  if (tail + 1024 + 4 * (size_t)a.stage_bytes > kMaxSmem) return cudaErrorInvalidValue;
   // Tiles on their way in a cluster: one multiplied, one stored, and those that the stages can hold
   // beyond (fewer leave the end of the work better shared out).
   a.tile_slots = 2 + (a.stages + a.kchunks - 1) / a.kchunks;
   if (a.tile_slots > kTileSlots) a.tile_slots = kTileSlots;
   a.wait_first = after_prep;
-  const size_t smem = 1024 + a.stages * stage_bytes(a.width) + kTailBytes;
+  const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + tail;
   switch (out_type) {
-    case VX_F32: return launch_typed<VX_F32>(maps, a, (int)units, smem, after_prep, st);
-    case VX_F16: return launch_typed<VX_F16>(maps, a, (int)units, smem, after_prep, st);
-    case VX_BF16: return launch_typed<VX_BF16>(maps, a, (int)units, smem, after_prep, st);
+    case VX_F32: return launch_out<VX_F32>(maps, a, (int)units, smem, after_prep, st);
+    case VX_F16: return launch_out<VX_F16>(maps, a, (int)units, smem, after_prep, st);
+    case VX_BF16: return launch_out<VX_BF16>(maps, a, (int)units, smem, after_prep, st);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -2679,11 +2679,12 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
   Scratch S(st);
   const int pitch = fp8_code_pitch(dim), scale_pitch = fp8_scale_pitch(dim);
   const uint8_t *q_codes = (const uint8_t*)q.p, *q_scales = q.scales;
-  const bool encode = q.type != VX_E4M3;
   const Fp8Tiling t = fp8_tiling(n, q.nq, row_off ? groups : 0, dev->sms);
   // Tiles are taken from a counter, but with 8 or fewer for each cluster in fixed turns: one query x
   // 100k x 768 rows (5.8 tiles each) 18.5 us in turns, 19.9 with the counter; 2M rows 246 and 223.
   const bool deal = row_off || t.tiles > 8 * (int64_t)(dev->sms / 2);
+  const bool resident = q.type != VX_E4M3 && !row_off && !deal && fp8_resident(q.nq, dim, t);
+  const bool encode = q.type != VX_E4M3 && !resident;
   const int firsts = dev->sms / 2;
   const size_t firsts_bytes = (size_t)firsts * 16, bounds_bytes = (size_t)groups * 16;
   const size_t off_bytes = row_off ? firsts_bytes + bounds_bytes + ((size_t)groups + 1) * sizeof(int64_t) : 0;
@@ -2721,7 +2722,7 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
   Fp8Maps maps{};
   if (!row_off) {
     fp8_map(&maps.rows[0], codes, n, pitch, t.tile_rows / 2);
-    fp8_map(&maps.queries[0], q_codes, q.nq, pitch, t.width / 2);
+    if (!resident) fp8_map(&maps.queries[0], q_codes, q.nq, pitch, t.width / 2);
   } else {
     for (int i = 0; i < 4; i++) {
       fp8_map(&maps.rows[i], codes, n, pitch, 128 >> i);
@@ -2731,6 +2732,12 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
   a.row_scales = scales;
   a.nrows = n;
   a.query_scales = q_scales;
+  if (resident) {
+    a.queries = q.p;
+    a.query_type = q.type;
+    a.dim = dim;
+    a.query_stride = q.stride;
+  }
   a.nq = q.nq;
   a.scale_words = scale_pitch / 4;
   a.kchunks = pitch / 128;
