@@ -12,8 +12,9 @@
 //   write  8 lanes take a block, 16 elements each in pieces of 16 (or 8) bytes, so that both sides are
 //          consecutive, the block's maximum is three shuffles away, and rows of any number of blocks
 //          fill the warps.  (A prefetched next block costs more in resident warps than it hides.)
+//          400k x 1024 fp32: 299-316 us, 6.5-6.9 TB/s; 100k x 768 bf16: 43 us, 5.4 TB/s.
 //   read   one warp takes up to 8 blocks of a row, 4 elements a lane and block, so that the wider
-//          side, its stores, is consecutive.
+//          side, its stores, is consecutive.  300k scattered rows x 1000 to fp16: 147-160 us, 5.7-6.2 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

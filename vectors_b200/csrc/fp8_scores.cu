@@ -274,7 +274,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // The launch before this one wrote the encoded queries, the groups' tile counts and the counter of
-  // tiles: every role waits for it where it needs them, and once in any case.
+  // tiles: every role waits for it before it needs them, and before a bounded wait that would take it
+  // in.  Stored rows and their scales are loaded without it, as far as there is room.
   const bool grouped = a.groups.row_off != nullptr;
   bool waited = !a.wait_first;
   auto wait_for_prep = [&]() {
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     }
     if (only_tile || ended) return false;
+    wait_for_prep();
     if (*abort_flag || !mbar_wait(&nfull[nslot], nphase, a.timeout_ns, abort_flag)) {
       give_up();
       return false;
@@ -333,11 +335,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       if (!rows) wait_for_prep();
+      int room = n_stages;
       Tile t;
       while (next_tile(t)) {
         const int count = rows ? t.half : t.width >> 1;  // operand rows of this CTA
         const int32_t y0 = (int32_t)(rows ? t.row : t.query) + (int)rank * count;
         for (int kc = 0; kc < a.kchunks; kc++) {
+          if (room-- == 0) wait_for_prep();
           if (!mbar_wait(&empty[stage], phase ^ 1u, a.timeout_ns, abort_flag)) {
             give_up();
             break;
@@ -385,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t resident_lo = (uint32_t)sw128_kmajor_desc(smem_addr(resident));
       const uint32_t resident_step = (uint32_t)(a.width / 2 * 128) >> 4;
       const uint64_t resident_ds = scale_block_desc(smem_addr(resident_scales));
+      wait_for_prep();
       if (kResident && !mbar_wait(encoded, 0, a.timeout_ns, abort_flag)) give_up();
       Tile t;
       for (uint32_t li = 0; next_tile(t); li++) {
@@ -450,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;
     const int first = (warp >> 2 & 1) * 32;  // this warp's 32-query groups: every other one
     const uint32_t tempty0 = mapa_shared(smem_addr(&tempty[0]), 0), nempty0 = mapa_shared(smem_addr(&nempty[0]), 0);
+    wait_for_prep();
     if constexpr (kResident) {
       if (a.query_type == VX_F32) encode_resident<float>(a, resident, resident_scales, rank);
       else if (a.query_type == VX_F16) encode_resident<__half>(a, resident, resident_scales, rank);
@@ -516,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int slot = 0;
     uint32_t sphase = 0;
     if (part > 0) wait_for_prep();
+    int room = kScaleSlots;
     Tile t;
     while ((part == 0 || !kResident) && __all_sync(0xFFFFFFFFu, next_tile(t))) {
       const int64_t first = (part == 0 ? t.row + rank * (uint32_t)t.half : t.query + (uint32_t)(part - 1) * 128u) + lane;
@@ -530,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       bool ok = true;
       for (int w = 0; w < slots_per_tile; w++) {
+        if (room-- == 0) wait_for_prep();
         ok = !*abort_flag && mbar_wait(&sempty[slot], sphase ^ 1u, a.timeout_ns, abort_flag);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) {
@@ -551,6 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 5) {
     // ---------------- slots that have landed go to the leader's MMA thread
     if (elect_one()) {
+      wait_for_prep();
       const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
       int slot = 0;
       uint32_t sphase = 0;
