@@ -381,8 +381,9 @@ VX_API int vx_fp8_read_device(int32_t device, const uint8_t* codes, const uint8_
  * out_stride elements apart, out_type VX_F32 / VX_F16 / VX_BF16.  Queries [nq][dim] of VX_F32 / VX_F16 /
  * VX_BF16, query_stride elements apart, are quantised as vx_fp8_write_device does; or they are stored
  * rows: query_type VX_E4M3 with their codes and query_scales (query_stride is not used).  Products are
- * exact and summed in fp32 (a result whose partial sums leave fp32's range is not finite); a NaN block
- * makes its query's or row's results NaN. */
+ * exact and summed in fp32 in one order (a query and a row give the same bits in every call; a result
+ * whose partial sums leave fp32's range is not finite); a NaN block makes its query's or row's results
+ * NaN. */
 VX_API int vx_fp8_scores_device(int32_t device, const void* queries, int32_t query_type, const uint8_t* query_scales,
                                 int64_t nq, int64_t query_stride, const uint8_t* codes, const uint8_t* scales,
                                 int64_t n, int32_t dim, void* out, int32_t out_type, int64_t out_stride, void* stream);

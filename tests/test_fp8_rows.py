@@ -710,6 +710,69 @@ def test_other_stream_and_graph():
         assert (np.abs(a.cpu().numpy() - dq @ dr.T) <= bound(dq, dr, "float32")).all()
 
 
+CAPTURED_FIRST = """
+import torch, vectors_b200 as vx
+x, q = torch.randn(3000, 300, device="cuda"), torch.randn(70, 300, device="cuda")
+codes, scales = vx.fp8_empty(4000, 300)
+slots = torch.randperm(4000, device="cuda")[:3000]
+out, few = torch.zeros(70, 4000, device="cuda"), torch.zeros(2, 4000, device="cuda")
+grouped = torch.zeros(70, 4000, device="cuda")
+qo, ro = torch.tensor([0, 30, 70], device="cuda"), torch.tensor([0, 1000, 4000], device="cuda")
+back = torch.zeros(3000, 300, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):  # the library's first calls in this process
+    vx.fp8_write_device(x, codes, scales, slots=slots)
+    vx.fp8_scores_device(q, codes, scales, out=out)
+    vx.fp8_scores_device(q[:2], codes, scales, out=few)
+    vx.fp8_scores_grouped_device(q, qo, codes, scales, ro, out=grouped)
+    vx.fp8_read_device(codes, scales, 300, slots=slots, out=back)
+g.replay()
+torch.cuda.synchronize()
+c, s = vx.fp8_empty(4000, 300)
+vx.fp8_write_device(x, c, s, slots=slots)
+want = vx.fp8_scores_device(q, c, s)
+assert torch.equal(codes.view(torch.uint8), c.view(torch.uint8)) and torch.equal(out, want)
+assert torch.equal(few, want[:2])
+assert torch.equal(grouped[:30, :1000], want[:30, :1000]) and torch.equal(grouped[30:, :3000], want[30:, 1000:])
+assert torch.equal(back, vx.fp8_read_device(c, s, 300, slots=slots))
+vx.fp8_check()
+print("captured first: ok")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured first: ok" in run.stdout, run.stdout + run.stderr
+
+
+@pytest.mark.gpu
+def test_results_of_a_pair_do_not_depend_on_the_call():
+    """The same query and row give the same bits as one of many queries, alone, from a stored copy, and in a
+    group: each result is one sum over dimensions in one order."""
+    import torch
+
+    x, q = torch.from_numpy(rows_of(5000, 700, 1)).cuda(), torch.from_numpy(rows_of(300, 700, 2)).cuda()
+    codes, scales = vx.fp8_empty(5000, 700)
+    vx.fp8_write_device(x, codes, scales)
+    many = vx.fp8_scores_device(q, codes, scales)
+    qc, qs = vx.fp8_empty(300, 700)
+    vx.fp8_write_device(q, qc, qs)
+    assert torch.equal(vx.fp8_scores_device(qc, codes, scales, query_scales=qs), many)
+    for n in (1, 20, 40, 100):
+        assert torch.equal(vx.fp8_scores_device(q[:n], codes, scales), many[:n])
+    assert torch.equal(vx.fp8_scores_device(q, codes[17:3001], scales[17:3001]), many[:, 17:3001])
+    off = torch.tensor([0, 7, 300], device="cuda")
+    rows = torch.tensor([0, 1234, 5000], device="cuda")
+    grouped = vx.fp8_scores_grouped_device(q, off, codes, scales, rows, max_rows=4000)
+    assert torch.equal(grouped[:7, :1234], many[:7, :1234]) and torch.equal(grouped[7:, :3766], many[7:, 1234:])
+
+
 @pytest.mark.gpu
 def test_two_threads_at_once():
     import threading
