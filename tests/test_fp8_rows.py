@@ -280,7 +280,7 @@ def test_blocks_with_nan_or_infinity_are_nan():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["int32", "int64"])
-@pytest.mark.parametrize("n", [1, 2, 37, 257, 512, 513, 5000])
+@pytest.mark.parametrize("n", [1, 2, 37, 257, 512, 513, 5000, 8192, 8193, 20000])
 def test_write_to_slots(n, kind):
     """Scattered, repeated and skipped slots: the last row of a slot is kept, other slots stay."""
     import torch
@@ -310,8 +310,8 @@ def test_write_to_slots(n, kind):
 def test_every_row_to_one_slot():
     import torch
 
-    x = rows_of(3000, 130, 9)
-    for n in (200, 1000, 3000):
+    x = rows_of(9000, 130, 9)
+    for n in (200, 1000, 3000, 9000):
         codes, scales = vx.fp8_empty(5, 130)
         vx.fp8_write_device(torch.from_numpy(x[:n]).cuda(), codes, scales, slots=torch.full((n,), 2, device="cuda"))
         c, s = encode(x[n - 1 : n])
