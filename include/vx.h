@@ -394,7 +394,8 @@ VX_API int vx_fp8_scores_device(int32_t device, const void* queries, int32_t que
  * past a group's rows, and rows of out in no group, are left as they are; a group's rows past max_rows are
  * not scored.  Offsets are clamped to the operands' sizes and an end below its start is an empty
  * group, so no offsets read or write out of range.  Groups may share rows; a query that several groups
- * name gets one of their results in each place. */
+ * name gets one of their results in each place.  With groups = 0 nothing is done and the offsets may be
+ * NULL. */
 VX_API int vx_fp8_scores_grouped_device(int32_t device, const void* queries, int32_t query_type,
                                         const uint8_t* query_scales, int64_t nq, int64_t query_stride,
                                         const int64_t* query_offsets, const uint8_t* codes, const uint8_t* scales,

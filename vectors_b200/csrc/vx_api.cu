@@ -2667,27 +2667,29 @@ void fp8_map(CUtensorMap* m, const uint8_t* codes, int64_t rows, int pitch, int 
   make_tmap(m, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pitch, rows, box_rows);
 }
 
-// The queries quantised if they are floats, the groups' tiles counted, and the product.
+// The queries quantised if they are floats, the groups' tiles counted, and the product.  groups < 0: not
+// grouped, every query with every row (the offsets say nothing: with no groups they may be null).
 int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const uint8_t* scales, int64_t n, int32_t dim,
                const int64_t* query_off, const int64_t* row_off, int64_t groups, void* out, int32_t out_type,
                int64_t out_stride, int64_t max_cols, cudaStream_t st) {
   Fp8Device* dev = nullptr;
   if (int s = fp8_device(device, &dev)) return s;
   if (int s = fp8_pending(dev)) return s;
-  if (n == 0 || q.nq == 0 || (row_off && (groups == 0 || max_cols == 0))) return VX_OK;
+  const bool grouped = groups >= 0;
+  if (n == 0 || q.nq == 0 || (grouped && (groups == 0 || max_cols == 0))) return VX_OK;
   DeviceScope here(device);
   Scratch S(st);
   const int pitch = fp8_code_pitch(dim), scale_pitch = fp8_scale_pitch(dim);
   const uint8_t *q_codes = (const uint8_t*)q.p, *q_scales = q.scales;
-  const Fp8Tiling t = fp8_tiling(n, q.nq, row_off ? groups : 0, dev->sms);
+  const Fp8Tiling t = fp8_tiling(n, q.nq, grouped ? groups : 0, dev->sms);
   // Tiles are taken from a counter, but with 8 or fewer for each cluster in fixed turns: one query x
   // 100k x 768 rows (5.8 tiles each) 18.5 us in turns, 19.9 with the counter; 2M rows 246 and 223.
-  const bool deal = row_off || t.tiles > 8 * (int64_t)(dev->sms / 2);
-  const bool resident = q.type != VX_E4M3 && !row_off && !deal && fp8_resident(q.nq, dim, t);
+  const bool deal = grouped || t.tiles > 8 * (int64_t)(dev->sms / 2);
+  const bool resident = q.type != VX_E4M3 && !deal && fp8_resident(q.nq, dim, t);
   const bool encode = q.type != VX_E4M3 && !resident;
   const int firsts = dev->sms / 2;
-  const size_t firsts_bytes = (size_t)firsts * 16, bounds_bytes = (size_t)groups * 16;
-  const size_t off_bytes = row_off ? firsts_bytes + bounds_bytes + ((size_t)groups + 1) * sizeof(int64_t) : 0;
+  const size_t firsts_bytes = (size_t)firsts * 16, bounds_bytes = grouped ? (size_t)groups * 16 : 0;
+  const size_t off_bytes = grouped ? firsts_bytes + bounds_bytes + ((size_t)groups + 1) * sizeof(int64_t) : 0;
   const size_t q_at = round_up(16 + off_bytes, 128);
   const size_t q_bytes = encode ? (size_t)q.nq * (pitch + scale_pitch) : 0;
   const bool prep = encode || deal;
@@ -2700,7 +2702,7 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
     uint8_t* buf = S.alloc<uint8_t>(q_at + q_bytes);
     Fp8WriteArgs w{};
     if (deal) a.next_tile = (unsigned long long*)buf;
-    if (row_off) {
+    if (grouped) {
       uint8_t* at = buf + 16;
       a.groups = Fp8Groups{row_off, query_off, groups, n, q.nq, max_cols, (int4*)(at + firsts_bytes),
                            (int64_t*)(at + firsts_bytes + bounds_bytes), (ulonglong2*)at, firsts};
@@ -2720,7 +2722,7 @@ int fp8_scores(int32_t device, const Fp8Queries& q, const uint8_t* codes, const 
     VX_LAUNCH(1, launch_fp8_prepare(w, a.groups, a.next_tile, st));
   }
   Fp8Maps maps{};
-  if (!row_off) {
+  if (!grouped) {
     fp8_map(&maps.rows[0], codes, n, pitch, t.tile_rows / 2);
     if (!resident) fp8_map(&maps.queries[0], q_codes, q.nq, pitch, t.width / 2);
   } else {
@@ -2810,7 +2812,7 @@ int vx_fp8_scores_device(int32_t device, const void* queries, int32_t query_type
     if (int s = fp8_check_store(codes, scales, n, dim)) return s;
     if (int s = fp8_check_queries(q, dim)) return s;
     if (int s = fp8_check_matrix("out", out, out_type, nq, n, out_stride)) return s;
-    return fp8_scores(device, q, codes, scales, n, dim, nullptr, nullptr, 0, out, out_type, out_stride, n,
+    return fp8_scores(device, q, codes, scales, n, dim, nullptr, nullptr, -1, out, out_type, out_stride, n,
                       (cudaStream_t)stream);
   });
 }
