@@ -28,3 +28,32 @@ def test_no_groups_and_no_offsets(max_rows):
         assert status == 0, N.last_error()
     vx.fp8_check()
     assert (out == -7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [1, 8, 74, 75, 200])
+def test_small_grouped_calls_one_after_another(groups):
+    """Fewer tiles than clusters (74 on a B200), as many, and a few more: hundreds of calls queued on three
+    streams, so that clusters of one call start where those of another have just ended."""
+    import torch
+
+    dim, per = 128, 7
+    q, x = rows_of(groups, dim, groups, 1.0), rows_of(groups * per, dim, groups + 1, 1.0)
+    codes, scales = _store(x)
+    qo, ro = np.arange(groups + 1), np.arange(groups + 1) * per
+    want, tol = _grouped_want(decode(*encode(q)), decode(_bytes(codes), scales.cpu().numpy()), qo, ro, per, 0.0)
+    tq, tqo, tro = torch.from_numpy(q).cuda(), torch.from_numpy(qo).cuda(), torch.from_numpy(ro).cuda()
+    qc, qs = _store(q)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    torch.cuda.synchronize()
+    for i in range(300):
+        with torch.cuda.stream(streams[i % 3]):
+            if i % 2:
+                outs.append(vx.fp8_scores_grouped_device(qc, tqo, codes, scales, tro, query_scales=qs, max_rows=per))
+            else:
+                outs.append(vx.fp8_scores_grouped_device(tq, tqo, codes, scales, tro, max_rows=per))
+    torch.cuda.synchronize()
+    vx.fp8_check()
+    assert (np.abs(outs[0].cpu().numpy() - want) <= tol).all()
+    assert all(torch.equal(o, outs[0]) for o in outs)

@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tile_slots = full + 64;  // 16-byte aligned
   uint32_t* tmem_slot = (uint32_t*)(tile_slots + 2 * kTileSlots);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  volatile uint32_t* tiles_sent = tmem_slot + 2;  // to this CTA, by the leader's tile warp
 
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(drained, 1);
     mbar_init(encoded, 16);  // the epilogue warps of both CTAs
     *abort_flag = 0;
+    *tiles_sent = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -582,38 +584,44 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (leader && !only_tile) {
     // ---------------- warp 7: tiles, to the same place in both CTAs
     if (grouped || a.next_tile) wait_for_prep();
-    Finder finder(a);
     const uint32_t at[2] = {mapa_shared(smem_addr(tile_slots), 0), mapa_shared(smem_addr(tile_slots), 1)};
     const uint32_t bar[2] = {mapa_shared(smem_addr(nfull), 0), mapa_shared(smem_addr(nfull), 1)};
-    // The cluster's first tile is known to every role.  With groups the number after the one in hand is on
-    // its way while the group is looked up.
-    unsigned long long taken = 0;
-    auto take = [&]() {
-      if (a.next_tile && lane == 0) taken = atomicAdd(a.next_tile, 1ull);
-    };
-    int64_t p = unit;
-    auto advance = [&]() {
-      if (!grouped) take();
-      p = a.next_tile ? units + (int64_t)__shfl_sync(0xFFFFFFFFu, taken, 0) : p + units;
+    uint32_t sent = 0;
+    Tile own;
+    if (next_tile(own)) {  // a cluster without a first tile has no role that would wait for a second
+      Finder finder(a);
+      // The cluster's first tile is known to every role.  With groups the number after the one in hand is on
+      // its way while the group is looked up.
+      unsigned long long taken = 0;
+      auto take = [&]() {
+        if (a.next_tile && lane == 0) taken = atomicAdd(a.next_tile, 1ull);
+      };
+      int64_t p = unit;
+      auto advance = [&]() {
+        if (!grouped) take();
+        p = a.next_tile ? units + (int64_t)__shfl_sync(0xFFFFFFFFu, taken, 0) : p + units;
+        if (grouped) take();
+      };
       if (grouped) take();
-    };
-    if (grouped) take();
-    advance();
-    for (int width = 1; width != 0; advance()) {
-      const Tile t = finder.find(p);
-      width = t.width;
-      const bool ok = mbar_wait(&nempty[nslot], nphase ^ 1u, a.timeout_ns, abort_flag);
-      if (!__all_sync(0xFFFFFFFFu, ok)) {
-        if (lane == 0) give_up();
-        break;
-      }
-      const ulonglong2 v = pack_tile(t);
-      if (lane < 2) store_cluster_16(at[lane] + (uint32_t)nslot * 16u, bar[lane] + (uint32_t)nslot * 8u, v.x, v.y);
-      if (++nslot == a.tile_slots) {
-        nslot = 0;
-        nphase ^= 1u;
+      advance();
+      for (int width = 1; width != 0; advance()) {
+        const Tile t = finder.find(p);
+        width = t.width;
+        const bool ok = mbar_wait(&nempty[nslot], nphase ^ 1u, a.timeout_ns, abort_flag);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          if (lane == 0) give_up();
+          break;
+        }
+        const ulonglong2 v = pack_tile(t);
+        if (lane < 2) store_cluster_16(at[lane] + (uint32_t)nslot * 16u, bar[lane] + (uint32_t)nslot * 8u, v.x, v.y);
+        sent++;
+        if (++nslot == a.tile_slots) {
+          nslot = 0;
+          nphase ^= 1u;
+        }
       }
     }
+    if (lane < 2) store_cluster_4(mapa_shared(smem_addr((const void*)tiles_sent), (uint32_t)lane), sent);
   }
 
   wait_for_prep();
@@ -622,6 +630,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+  // Only its mbarrier tells that a tile's asynchronous store has landed, not the cluster's barrier, and roles
+  // that gave up have not looked: a CTA stays until the last tile sent to each slot is there.
+  if (warp == 7 && lane < a.tile_slots && (uint32_t)lane < *tiles_sent) {
+    const uint32_t turn = (*tiles_sent - 1 - (uint32_t)lane) / (uint32_t)a.tile_slots;
+    const uint64_t until = globaltimer_ns() + 2000000ull;
+    while (!mbar_try_wait(&nfull[lane], turn & 1u) && globaltimer_ns() < until) {
+    }
   }
 }
 

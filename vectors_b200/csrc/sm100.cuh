@@ -238,6 +238,10 @@ __device__ __forceinline__ void store_cluster_16(uint32_t dst, uint32_t bar, uin
                "l"(y), "r"(bar)
                : "memory");
 }
+// 4 bytes into the shared memory of a CTA of the cluster, there after the next cluster_sync.
+__device__ __forceinline__ void store_cluster_4(uint32_t dst, uint32_t x) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst), "r"(x) : "memory");
+}
 // 4-byte copy from global to shared memory (zero when !valid), and an arrival on `bar` when all of
 // this thread's copies so far have landed.
 __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* src, bool valid) {
