@@ -57,3 +57,26 @@ def test_small_grouped_calls_one_after_another(groups):
     vx.fp8_check()
     assert (np.abs(outs[0].cpu().numpy() - want) <= tol).all()
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [128, 512, 640, 1500, 1664, 4000])
+def test_short_calls_of_every_pipeline_depth(dim):
+    """Products of fewer chunks than the pipeline has stages, as many and more, queued on three streams so that
+    clusters of one call start where those of another have just ended."""
+    import torch
+
+    q, x = rows_of(50, dim, 3, 1.0), rows_of(700, dim, 4, 1.0)
+    codes, scales = _store(x)
+    qc, qs = _store(q)
+    dq, dr = decode(*encode(q)), decode(_bytes(codes), scales.cpu().numpy())
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(150):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(vx.fp8_scores_device(qc, codes, scales, query_scales=qs))
+    torch.cuda.synchronize()
+    vx.fp8_check()
+    assert (np.abs(got[0].cpu().numpy() - dq @ dr.T) <= bound(dq, dr, "float32")).all()
+    assert all(torch.equal(g, got[0]) for g in got)

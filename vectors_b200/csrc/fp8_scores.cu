@@ -372,6 +372,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      // The hand-backs of the last stages arrive here too (a stage's loads have landed by then): this CTA
+      // stays for them.
+      if (rows) {
+        wait_for_prep();
+        for (int i = 0; i < n_stages && !*abort_flag; i++) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, a.timeout_ns, abort_flag)) give_up();
+          if (++stage == n_stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
       if (*abort_flag) {
         // Let the loads already issued land before the cluster's shared memory is released.
         const uint64_t until = globaltimer_ns() + 2000000ull;
@@ -444,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         mma_commit_pair_mc(&tfull[acc], (uint16_t)0x3);
       }
-      if (*abort_flag) {  // MMAs in flight end before their TMEM and shared memory are released
+      {  // MMAs in flight end before their TMEM and shared memory are released, whoever else has given up
         mma_commit_pair_mc(drained, (uint16_t)0x1);
         const uint64_t until = globaltimer_ns() + 2000000ull;
         while (!mbar_try_wait(drained, 0) && globaltimer_ns() < until) {
@@ -556,6 +568,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!ok) break;
+    }
+    if (part == 0) {  // the last slots' hand-backs, as above
+      wait_for_prep();
+      for (int i = 0; i < kScaleSlots; i++) {
+        const bool ok = !*abort_flag && mbar_wait(&sempty[slot], sphase ^ 1u, a.timeout_ns, abort_flag);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+          if (lane == 0) give_up();
+          break;
+        }
+        if (++slot == kScaleSlots) {
+          slot = 0;
+          sphase ^= 1u;
+        }
+      }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 5) {
