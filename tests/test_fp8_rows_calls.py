@@ -80,3 +80,25 @@ def test_short_calls_of_every_pipeline_depth(dim):
     vx.fp8_check()
     assert (np.abs(got[0].cpu().numpy() - dq @ dr.T) <= bound(dq, dr, "float32")).all()
     assert all(torch.equal(g, got[0]) for g in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq, dim", [(1, 768), (20, 500), (64, 256)])
+def test_few_queries_that_change_from_call_to_call(nq, dim):
+    """Few float queries are quantised inside the product, by both CTAs of each cluster for its tensor cores:
+    calls in a row on other queries each see their own (a stale code or scale is another call's)."""
+    import torch
+
+    x = rows_of(30000, dim, 1)
+    codes, scales = _store(x)
+    sets = [torch.from_numpy(rows_of(nq, dim, 10 + s)).cuda() for s in range(4)]
+    want = []
+    for q in sets:
+        qc, qs = vx.fp8_empty(nq, dim)
+        vx.fp8_write_device(q, qc, qs)
+        want.append(vx.fp8_scores_device(qc, codes, scales, query_scales=qs))
+    for n in (30000, 1000):
+        got = [vx.fp8_scores_device(sets[i % 4], codes[:n], scales[:n]) for i in range(100)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want[i % 4][:, :n]) for i, g in enumerate(got))
+    vx.fp8_check()

@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t resident_step = (uint32_t)(a.width / 2 * 128) >> 4;
       const uint64_t resident_ds = scale_block_desc(smem_addr(resident_scales));
       wait_for_prep();
-      if (kResident && !mbar_wait(encoded, 0, a.timeout_ns, abort_flag)) give_up();
+      if (kResident && !mbar_wait<true>(encoded, 0, a.timeout_ns, abort_flag)) give_up();
       Tile t;
       for (uint32_t li = 0; next_tile(t); li++) {
         const int acc = (int)(li & 1);
@@ -476,7 +476,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       else encode_resident<__nv_bfloat16>(a, resident, resident_scales, rank);
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive_pair(mapa_shared(smem_addr(encoded), 0));
+      // released and acquired at cluster scope: plain stores of either CTA, announced to a thread of one
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_addr(encoded), 0));
     }
     for (uint32_t li = 0;; li++) {
       Tile t;
