@@ -235,7 +235,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tile_slots = full + 64;  // 16-byte aligned
   uint32_t* tmem_slot = (uint32_t*)(tile_slots + 2 * kTileSlots);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  volatile uint32_t* tiles_sent = tmem_slot + 2;  // to this CTA, by the leader's tile warp
 
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -264,7 +263,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(drained, 1);
     mbar_init(encoded, 16);  // the epilogue warps of both CTAs
     *abort_flag = 0;
-    *tiles_sent = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -372,12 +370,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // The hand-backs of the last stages arrive here too (a stage's loads have landed by then): this CTA
-      // stays for them.
       if (rows) {
+        // tcgen05.commit's arrivals come by themselves, and the cluster's barrier does not wait for them: this
+        // CTA stays for the last hand-back of each stage (the epilogue takes longer)
         wait_for_prep();
-        for (int i = 0; i < n_stages && !*abort_flag; i++) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, a.timeout_ns, abort_flag)) give_up();
+        for (int i = 0; i < n_stages; i++) {
+          mbar_settle(&empty[stage], phase ^ 1u);
           if (++stage == n_stages) {
             stage = 0;
             phase ^= 1u;
@@ -456,12 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         mma_commit_pair_mc(&tfull[acc], (uint16_t)0x3);
       }
-      {  // MMAs in flight end before their TMEM and shared memory are released, whoever else has given up
-        mma_commit_pair_mc(drained, (uint16_t)0x1);
-        const uint64_t until = globaltimer_ns() + 2000000ull;
-        while (!mbar_try_wait(drained, 0) && globaltimer_ns() < until) {
-        }
-      }
+      // MMAs in flight end before their TMEM and shared memory are released, whoever else has given up
+      mma_commit_pair_mc(drained, (uint16_t)0x1);
+      mbar_settle(drained, 0);
     }
   } else if (warp >= 8) {
     // ---------------- epilogue: one stored row per lane, one query per TMEM column
@@ -570,14 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
     }
-    if (part == 0) {  // the last slots' hand-backs, as above
+    if (part == 0) {  // the last hand-back of each slot, as of the stages
       wait_for_prep();
       for (int i = 0; i < kScaleSlots; i++) {
-        const bool ok = !*abort_flag && mbar_wait(&sempty[slot], sphase ^ 1u, a.timeout_ns, abort_flag);
-        if (!__all_sync(0xFFFFFFFFu, ok)) {
-          if (lane == 0) give_up();
-          break;
-        }
+        mbar_settle(&sempty[slot], sphase ^ 1u);
         if (++slot == kScaleSlots) {
           slot = 0;
           sphase ^= 1u;
@@ -613,7 +604,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (grouped || a.next_tile) wait_for_prep();
     const uint32_t at[2] = {mapa_shared(smem_addr(tile_slots), 0), mapa_shared(smem_addr(tile_slots), 1)};
     const uint32_t bar[2] = {mapa_shared(smem_addr(nfull), 0), mapa_shared(smem_addr(nfull), 1)};
-    uint32_t sent = 0;
     Tile own;
     if (next_tile(own)) {  // a cluster without a first tile has no role that would wait for a second
       Finder finder(a);
@@ -641,14 +631,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const ulonglong2 v = pack_tile(t);
         if (lane < 2) store_cluster_16(at[lane] + (uint32_t)nslot * 16u, bar[lane] + (uint32_t)nslot * 8u, v.x, v.y);
-        sent++;
         if (++nslot == a.tile_slots) {
           nslot = 0;
           nphase ^= 1u;
         }
       }
     }
-    if (lane < 2) store_cluster_4(mapa_shared(smem_addr((const void*)tiles_sent), (uint32_t)lane), sent);
   }
 
   wait_for_prep();
@@ -658,12 +646,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, kTmemCols);
   }
-  // Only its mbarrier tells that a tile's asynchronous store has landed, not the cluster's barrier, and roles
-  // that gave up have not looked: a CTA stays until the last tile sent to each slot is there.
-  if (warp == 7 && lane < a.tile_slots && (uint32_t)lane < *tiles_sent) {
-    const uint32_t turn = (*tiles_sent - 1 - (uint32_t)lane) / (uint32_t)a.tile_slots;
+  // Nor does the cluster's barrier wait for asynchronous stores (tiles).  A role that ends in order has seen
+  // them all; a CTA that gave up stays for what the other may have sent it until then.
+  if (warp == 7 && *abort_flag) {
     const uint64_t until = globaltimer_ns() + 2000000ull;
-    while (!mbar_try_wait(&nfull[lane], turn & 1u) && globaltimer_ns() < until) {
+    while (globaltimer_ns() < until) {
     }
   }
 }

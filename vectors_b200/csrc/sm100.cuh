@@ -73,6 +73,16 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
   }
   return true;
 }
+// The same for an arrival that is on its way: 2 ms from the 256th poll, whoever has given up.
+__device__ __forceinline__ void mbar_settle(uint64_t* bar, uint32_t parity) {
+  uint64_t until = 0;
+  for (uint32_t spins = 1; !mbar_try_wait(bar, parity); spins++) {
+    if ((spins & 255u) != 0) continue;
+    const uint64_t now = globaltimer_ns();
+    if (until == 0) until = now + 2000000ull;
+    else if (now > until) return;
+  }
+}
 
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
@@ -250,10 +260,6 @@ __device__ __forceinline__ void store_cluster_16(uint32_t dst, uint32_t bar, uin
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(dst), "l"(x),
                "l"(y), "r"(bar)
                : "memory");
-}
-// 4 bytes into the shared memory of a CTA of the cluster, there after the next cluster_sync.
-__device__ __forceinline__ void store_cluster_4(uint32_t dst, uint32_t x) {
-  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(dst), "r"(x) : "memory");
 }
 // 4-byte copy from global to shared memory (zero when !valid), and an arrival on `bar` when all of
 // this thread's copies so far have landed.
