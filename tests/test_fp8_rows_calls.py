@@ -102,3 +102,22 @@ def test_few_queries_that_change_from_call_to_call(nq, dim):
         torch.cuda.synchronize()
         assert all(torch.equal(g, want[i % 4][:, :n]) for i, g in enumerate(got))
     vx.fp8_check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq, n, dim", [(3, 9000, 2048), (200, 3000, 4096), (130, 5000, 600)])
+def test_scales_that_change_from_slot_to_slot(nq, n, dim):
+    """Scales far apart from block to block and from call to call, copied by both CTAs of each cluster for its
+    tensor cores: a scale of an earlier slot or call would be off by powers of two."""
+    import torch
+
+    stores = [_store(rows_of(n, dim, 30 + s, 6.0)) for s in range(2)]
+    queries = [_store(rows_of(nq, dim, 40 + s, 6.0)) for s in range(2)]
+    got = [vx.fp8_scores_device(queries[i % 2][0], *stores[i // 2 % 2], query_scales=queries[i % 2][1]) for i in range(60)]
+    torch.cuda.synchronize()
+    vx.fp8_check()
+    for i in range(4):
+        dq = decode(_bytes(queries[i % 2][0]), queries[i % 2][1].cpu().numpy())
+        dr = decode(_bytes(stores[i // 2][0]), stores[i // 2][1].cpu().numpy())
+        assert (np.abs(got[i].cpu().numpy() - dq @ dr.T) <= bound(dq, dr, "float32")).all()
+        assert all(torch.equal(g, got[i]) for g in got[i::4])

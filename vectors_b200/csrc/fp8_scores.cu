@@ -26,8 +26,10 @@
 // gives four chunks' exponents, which go to TMEM as they are (the descriptor's scale id picks the
 // byte).  Three warps copy them to shared memory (cp.async), a fourth hands a slot that has landed
 // to the MMA thread, which copies it to TMEM (tcgen05.cp) in the tensor core's own order ahead of
-// its MMAs.  (Stored from registers with tcgen05.st, or handed over with a release at cluster scope,
-// a slot took 1,400-2,000 cycles, more than its MMAs.)
+// its MMAs.  (Stored from registers with tcgen05.st, or handed over with a plain release at cluster
+// scope, a slot took 1,400-2,000 cycles, more than its MMAs: 2M x 768, one query, 256 -> 349 us.  The
+// second CTA's slots are released by the completion of an asynchronous store instead, which costs
+// nothing that could be measured.)
 //
 // Tiles.  Clusters take tiles from a counter where there are many: with large results the SMs' shares of
 // the write bandwidth differ (the slowest unit of 1000 x 100k x 128 in fixed turns took 87 us with the
@@ -287,6 +289,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 1;
     record_error(a.err, kDevWaitTimeout);
   };
+  // Shared memory of this CTA that the pair's tensor cores may read, announced to the leader's MMA thread:
+  // released and acquired at cluster scope.
+  const uint32_t leader_bars = mapa_shared(smem_addr(full), 0), nothing = mapa_shared(smem_addr(tmem_slot + 2), 0);
+  auto announce = [&](uint64_t* bar) {
+    if (leader) mbar_arrive(bar);
+    else mbar_arrive_cluster_async(leader_bars + (uint32_t)((uint8_t*)bar - (uint8_t*)full), nothing);
+  };
   // Each role takes the tiles in order; false: no more, or given up.  A cluster's first tile is the one of
   // its number: without groups known at once, with groups one of those that the launch before this one
   // left.
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (only_tile || ended) return false;
     wait_for_prep();
-    if (*abort_flag || !mbar_wait(&nfull[nslot], nphase, a.timeout_ns, abort_flag)) {
+    if (*abort_flag || !mbar_wait<true>(&nfull[nslot], nphase, a.timeout_ns, abort_flag)) {
       give_up();
       return false;
     }
@@ -415,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t idesc0 = idesc_mxf8(256, t.width, 0);
         bool ok = true;
         for (int kc = 0; kc < a.kchunks && ok; kc += 4) {  // a scale slot's chunks
-          if (!mbar_wait(&sfull[slot], sphase, a.timeout_ns, abort_flag)) {
+          if (!mbar_wait<true>(&sfull[slot], sphase, a.timeout_ns, abort_flag)) {
             ok = false;
             break;
           }
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int sub = 0; sub < 4; sub++) {
             if (kc + sub >= a.kchunks) break;
-            if (!mbar_wait(&full[stage], phase, a.timeout_ns, abort_flag)) {
+            if (!mbar_wait<true>(&full[stage], phase, a.timeout_ns, abort_flag)) {
               ok = false;
               break;
             }
@@ -471,8 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       else encode_resident<__nv_bfloat16>(a, resident, resident_scales, rank);
       fence_proxy_async();
       __syncwarp();
-      // released and acquired at cluster scope: plain stores of either CTA, announced to a thread of one
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_addr(encoded), 0));
+      if (lane == 0) announce(encoded);
     }
     for (uint32_t li = 0;; li++) {
       Tile t;
@@ -580,7 +588,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- slots that have landed go to the leader's MMA thread
     if (elect_one()) {
       wait_for_prep();
-      const uint32_t sfull0 = mapa_shared(smem_addr(&sfull[0]), 0);
       int slot = 0;
       uint32_t sphase = 0;
       Tile t;
@@ -591,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           fence_proxy_async();
-          mbar_arrive_pair(sfull0 + (uint32_t)(slot * 8));
+          announce(&sfull[slot]);
           if (++slot == kScaleSlots) {
             slot = 0;
             sphase ^= 1u;

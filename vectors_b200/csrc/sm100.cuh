@@ -248,17 +248,21 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// The same with the default release (CTA scope): for shared memory of this CTA that its own barriers
-// have shown to be written, and that the pair's tensor cores read once the arrival is seen.
-__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
 // 16 bytes into the shared memory of a CTA of the cluster, counted on a barrier of that CTA (whose
 // phase also gets this thread's arrival).
 __device__ __forceinline__ void store_cluster_16(uint32_t dst, uint32_t bar, uint64_t x, uint64_t y) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], 16;" ::"r"(bar) : "memory");
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(dst), "l"(x),
                "l"(y), "r"(bar)
+               : "memory");
+}
+// Arrival on a barrier of a CTA of the cluster that releases, at cluster scope, what this thread has written
+// and seen: the completion of an asynchronous store (of nothing, to the 8 bytes at `dst`) is such a release,
+// comes after the thread's accesses before it, and holds nobody up, where mbar_arrive_cluster waits for
+// the SM's memory traffic.
+__device__ __forceinline__ void mbar_arrive_cluster_async(uint32_t bar, uint32_t dst) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], 8;" ::"r"(bar) : "memory");
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(dst), "l"(0ull), "r"(bar)
                : "memory");
 }
 // 4-byte copy from global to shared memory (zero when !valid), and an arrival on `bar` when all of
