@@ -121,3 +121,41 @@ def test_scales_that_change_from_slot_to_slot(nq, n, dim):
         dr = decode(_bytes(stores[i // 2][0]), stores[i // 2][1].cpu().numpy())
         assert (np.abs(got[i].cpu().numpy() - dq @ dr.T) <= bound(dq, dr, "float32")).all()
         assert all(torch.equal(g, got[i]) for g in got[i::4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("queries", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("view", ["whole", "half_aligned", "shifted"])
+@pytest.mark.parametrize("groups, nq, n, dim", [(6, 700, 1500, 256), (40, 90, 3000, 200), (3, 5, 1100, 640), (300, 2000, 1200, 96)])
+def test_grouped_values_of_every_type(groups, nq, n, dim, view, queries, out):
+    """Queries of each type, with rows that every load width starts at, and results of each type: the values of
+    every group, what lies past a group's rows kept in a given result and zero in a new one."""
+    import torch
+
+    r = np.random.default_rng(groups)
+    q, x = rows_of(nq, dim + 4, groups, 1.0), rows_of(n, dim, groups + 1, 1.0)
+    # elements from one query to the next and the first one's place: 16-byte loads, 8-byte loads, single elements
+    wide = torch.from_numpy(q).cuda().to(_dtype(queries))
+    tq = {"whole": wide[:, :dim].contiguous(), "half_aligned": wide[:, 4:], "shifted": wide[:, 1 : dim + 1]}[view]
+    qo = np.sort(np.concatenate([[0, nq], r.integers(0, nq + 1, groups - 1)]))
+    ro = np.sort(np.concatenate([[0, n], r.integers(0, n + 1, groups - 1)]))
+    codes, scales = _store(x)
+    dq, dr = decode(*encode(tq.float().cpu().numpy())), decode(_bytes(codes), scales.cpu().numpy())
+    width = int((ro[1:] - ro[:-1]).max())
+    tqo, tro = torch.from_numpy(qo).cuda(), torch.from_numpy(ro).cuda()
+    value = np.zeros((nq, width))
+    tol, inside = np.zeros((nq, width)), np.zeros((nq, width), bool)
+    for g in range(groups):
+        a, b, c, d = qo[g], qo[g + 1], ro[g], ro[g + 1]
+        if a < b and c < d:
+            value[a:b, : d - c] = dq[a:b] @ dr[c:d].T
+            tol[a:b, : d - c] = bound(dq[a:b], dr[c:d], out)
+            inside[a:b, : d - c] = True
+    given = torch.full((nq, width), -3.0, dtype=_dtype(out), device="cuda")
+    fresh = vx.fp8_scores_grouped_device(tq, tqo, codes, scales, tro, max_rows=width, dtype=_dtype(out))
+    assert vx.fp8_scores_grouped_device(tq, tqo, codes, scales, tro, out=given) is given
+    for got, past in ((given, -3.0), (fresh, 0.0)):
+        assert got.dtype == _dtype(out)
+        err = np.abs(got.float().cpu().numpy().astype(np.float64) - np.where(inside, value, past))
+        assert (err <= tol).all(), (err.max(), np.argwhere(err > tol)[:5])
