@@ -10,6 +10,40 @@ import vectors_b200._native as N
 from tests.test_fp8_rows import _bytes, _dtype, _grouped_want, _store, bound, decode, encode, rows_of
 
 
+STAR = """
+import sys
+if {blocked}:
+    sys.modules["torch"] = None  # as where it is not installed: importing it raises ImportError
+from vectors_b200 import *
+import vectors_b200
+assert {blocked} or "torch" not in sys.modules
+assert all(n in globals() for n in vectors_b200.__all__) and "FlatScanAdapter" in globals()
+try:
+    assert fp8_pitch(513) == (640, 8) == vectors_b200.fp8_pitch(513)
+    assert not {blocked} and "torch" in sys.modules
+    assert vectors_b200.fp8_pitch is vectors_b200.fp8.fp8_pitch
+    try:
+        fp8_empty(capacity=-1, dim=100, device="cpu")
+    except IllegalArgumentException:
+        print("star: ok")
+except ImportError:
+    assert {blocked}
+    print("star: ok")
+"""
+
+
+@pytest.mark.parametrize("blocked", [False, True])
+def test_star_import_without_torch(blocked):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", STAR.format(blocked=blocked)], cwd=root, capture_output=True, text=True,
+                         timeout=300)
+    assert run.returncode == 0 and "star: ok" in run.stdout, run.stdout + run.stderr
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("max_rows", [5, 0])
 def test_no_groups_and_no_offsets(max_rows):

@@ -4,6 +4,8 @@ The scans (FLAT exact search, the SQ8 / FP16 / sign-bit BQ quantized scans and t
 list scan) run as hand-written CUDA kernels in ``libvx.so``; this package is the host-side
 mirror of the reference's index SPI over that library's C ABI (include/vx.h).
 """
+import sys as _sys
+
 from ._native import VxError, device_count, kernel_launches, lib  # noqa: F401
 from .index_spi import (  # noqa: F401
     FlatScanAdapter,
@@ -58,10 +60,21 @@ _FP8 = frozenset(n for n in __all__ if n.startswith("fp8_"))
 
 
 def __getattr__(name):
-    """The 8-bit row functions (fp8.py) work on torch tensors; torch is imported with the first of them."""
-    if name in _FP8:
-        from . import fp8
+    """The 8-bit row functions (fp8.py) work on torch tensors.  Where torch is not imported yet, each is a
+    stand-in that imports it when called: a star import needs no torch and loads none."""
+    if name not in _FP8:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    if _sys.modules.get("torch") is None:
 
-        globals().update({n: getattr(fp8, n) for n in _FP8})
-        return globals()[name]
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+        def call(*args, **kwargs):
+            from . import fp8
+
+            return getattr(fp8, name)(*args, **kwargs)
+
+        call.__name__ = call.__qualname__ = name
+        call.__doc__ = f"``{__name__}.fp8.{name}``, which imports torch."
+        return call
+    from . import fp8
+
+    globals().update({n: getattr(fp8, n) for n in _FP8})
+    return globals()[name]
