@@ -44,6 +44,64 @@ def test_star_import_without_torch(blocked):
     assert run.returncode == 0 and "star: ok" in run.stdout, run.stdout + run.stderr
 
 
+class _OnDevice:
+    """A host tensor that says it is on device 0: what these calls refuse, they refuse before any use of it."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return self.t.is_contiguous()
+
+    def contiguous(self):
+        return self
+
+
+def _refused(monkeypatch, call):
+    """The message of a call that is refused before it reaches the library."""
+    import vectors_b200.fp8 as fp8
+
+    monkeypatch.setattr(fp8, "_call", lambda name: pytest.fail(f"{name} was called"))
+    monkeypatch.setattr(fp8, "_raw_stream", lambda device: 0)
+    with pytest.raises(vx.IllegalArgumentException) as e:
+        call()
+    return str(e.value)
+
+
+def _host_store(capacity, dim):
+    codes, scales = vx.fp8_empty(capacity, dim, device="cpu")
+    return _OnDevice(codes), _OnDevice(scales)
+
+
+@pytest.mark.parametrize("first", [-1, 8, 1 << 31, 1 << 63, 1 << 64, -(1 << 64), (1 << 64) + 2])
+def test_first_row_out_of_the_store(monkeypatch, first):
+    """Also numbers that 64 bits would wrap into the store."""
+    import torch
+
+    codes, scales = _host_store(10, 100)
+    rows = _OnDevice(torch.zeros(3, 100))
+    assert "store of 10" in _refused(monkeypatch, lambda: vx.fp8_write_device(rows, codes, scales, first=first))
+    out = _OnDevice(torch.zeros(3, 100))
+    assert "store of 10" in _refused(monkeypatch, lambda: vx.fp8_read_device(codes, scales, 100, first=first, count=3, out=out))
+
+
+def test_first_row_with_slots(monkeypatch):
+    import torch
+
+    codes, scales = _host_store(10, 100)
+    rows, slots = _OnDevice(torch.zeros(3, 100)), _OnDevice(torch.zeros(3, dtype=torch.int64))
+    message = _refused(monkeypatch, lambda: vx.fp8_write_device(rows, codes, scales, slots=slots, first=2))
+    assert "exclude" in message
+    message = _refused(monkeypatch, lambda: vx.fp8_read_device(codes, scales, 100, slots=slots, first=2, out=rows))
+    assert "exclude" in message
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("max_rows", [5, 0])
 def test_no_groups_and_no_offsets(max_rows):

@@ -134,6 +134,15 @@ def _slots(slots, device: int):
     return slots.contiguous()
 
 
+def _place(first: int, n: int, capacity: int, slots) -> None:
+    """Rows first .. first + n - 1 must lie in the store; with slots there is no first row."""
+    if slots is not None:
+        if first != 0:
+            raise IllegalArgumentException(f"first ({first}) and slots exclude each other")
+    elif first < 0 or n > capacity - first:
+        raise IllegalArgumentException(f"rows [{first}, {first + n}) do not fit a store of {capacity}")
+
+
 def _on_stream(stream: int, codes):
     """Makes a raw stream current, so that what a call allocates or copies belongs to it."""
     device = codes.get_device() if isinstance(codes, torch.Tensor) and codes.is_cuda else None
@@ -143,7 +152,7 @@ def _on_stream(stream: int, codes):
 def fp8_write_device(rows, codes, scales, slots=None, first: int = 0, stream=None) -> None:
     """Quantises rows [n][dim] (float32 / float16 / bfloat16) into a store: row i into slot
     ``slots[i]`` (int32 or int64; outside [0, capacity) the row is skipped; of rows that name the same
-    slot the last is kept), or into ``first + i`` without slots.  Other rows stay as they are.  Writes
+    slot the last is kept), or into ``first + i`` (``first`` is for calls without slots).  Other rows stay as they are.  Writes
     that overlap on other streams are ordered by the caller."""
     if stream is not None:
         with _on_stream(stream, codes):
@@ -158,6 +167,7 @@ def fp8_write_device(rows, codes, scales, slots=None, first: int = 0, stream=Non
         if slots.shape[0] != n:
             raise IllegalArgumentException(f"slots must be [{n}], got {list(slots.shape)}")
         at, size = slots.data_ptr(), slots.element_size()
+    _place(first, n, capacity, slots)
     _check(_call("vx_fp8_write_device")(device, rows.data_ptr(), _type_of(rows, "rows"), n, dim, step, at, size, first,
                                         codes.data_ptr(), scales.data_ptr(), capacity, _raw_stream(device)))
 
@@ -181,6 +191,7 @@ def fp8_read_device(codes, scales, dim: int, slots=None, first: int = 0, count: 
         n = capacity - first if count is None else count
     if n < 0 or (count is not None and count != n):
         raise IllegalArgumentException(f"count {count} does not match the {n} rows asked for")
+    _place(first, n, capacity, slots)
     out, step = _out(out, n, dim, dtype, codes, False)
     _check(_call("vx_fp8_read_device")(device, codes.data_ptr(), scales.data_ptr(), capacity, dim, at, size, first, n,
                                        out.data_ptr(), _type_of(out, "out"), step, _raw_stream(device)))
