@@ -251,3 +251,48 @@ def test_grouped_values_of_every_type(groups, nq, n, dim, view, queries, out):
         assert got.dtype == _dtype(out)
         err = np.abs(got.float().cpu().numpy().astype(np.float64) - np.where(inside, value, past))
         assert (err <= tol).all(), (err.max(), np.argwhere(err > tol)[:5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", ["write", "read", "few", "many", "stored", "grouped", "check"])
+def test_first_cuda_call_of_a_thread(call):
+    """Each function as the first CUDA call that a thread makes (it has no current context yet)."""
+    import threading
+
+    import torch
+
+    x, q = torch.from_numpy(rows_of(500, 100, 1)).cuda(), torch.from_numpy(rows_of(300, 100, 2)).cuda()
+    codes, scales = vx.fp8_empty(500, 100)
+    vx.fp8_write_device(x, codes, scales)
+    c2, s2 = vx.fp8_empty(500, 100)
+    off = torch.tensor([0, 300], device="cuda"), torch.tensor([0, 500], device="cuda")
+    back, out = torch.empty_like(x), torch.empty(300, 500, device="cuda")
+    calls = {"write": lambda: vx.fp8_write_device(x, c2, s2), "read": lambda: vx.fp8_read_device(codes, scales, 100, out=back),
+             "few": lambda: vx.fp8_scores_device(q[:3], codes, scales, out=out[:3]),
+             "many": lambda: vx.fp8_scores_device(q, codes, scales, out=out),
+             "stored": lambda: vx.fp8_scores_device(codes[:300], codes, scales, query_scales=scales[:300], out=out),
+             "grouped": lambda: vx.fp8_scores_grouped_device(q, off[0], codes, scales, off[1], out=out),
+             "check": lambda: vx.fp8_check()}
+    torch.cuda.synchronize()
+    failed = []
+
+    def work():
+        try:
+            calls[call]()
+        except Exception as e:
+            failed.append(e)
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert not failed
+    if call == "write":
+        assert torch.equal(c2.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(s2, scales)
+    elif call == "read":
+        assert torch.equal(back, vx.fp8_read_device(codes, scales, 100))
+    elif call in ("few", "many", "grouped"):
+        n = 3 if call == "few" else 300
+        assert torch.equal(out[:n], vx.fp8_scores_device(q[:n], codes, scales))
+    elif call == "stored":
+        assert torch.equal(out, vx.fp8_scores_device(codes[:300], codes, scales, query_scales=scales[:300]))

@@ -2546,13 +2546,15 @@ int vx_merge_shards_device(int32_t device, int32_t nshards, const int64_t* d_off
 namespace vx {
 namespace {
 
-// Makes `device` current for a call and puts the caller's device back afterwards.
+// Makes `device` current for a call and puts the caller's device back afterwards.  Set even where it is the
+// thread's device already: a thread that has made no CUDA call yet has its device's number but no context,
+// without which tensor maps cannot be encoded.
 struct DeviceScope {
   int before = -1;
   explicit DeviceScope(int device) {
     if (cudaGetDevice(&before) != cudaSuccess) before = -1;
     if (before == device) before = -1;
-    else VX_CUDA(cudaSetDevice(device));
+    VX_CUDA(cudaSetDevice(device));
   }
   ~DeviceScope() {
     if (before >= 0) cudaSetDevice(before);
