@@ -117,6 +117,9 @@ VX_API int vx_debug_fail_next(int32_t status);
  * scan returns when one of its waits runs out.  The context stays usable.  No counterpart in the
  * reference. */
 VX_API int vx_debug_wait_timeout(int32_t device, int32_t timeout_ms);
+/* Test hook: the same kernel queued on `stream` in the place of an 8-bit score product whose wait runs out:
+ * the next vx_fp8_scores* call on the device or vx_fp8_check after it returns VX_ERR_DEVICE_TIMEOUT. */
+VX_API int vx_debug_fp8_wait_timeout(int32_t device, int32_t timeout_ms, void* stream);
 
 /* ---- index construction (the handle owns device copies; inputs are not retained) ----- */
 /* Input arrays of the build calls may be host or device memory (unified addressing), except
@@ -403,7 +406,9 @@ VX_API int vx_fp8_scores_grouped_device(int32_t device, const void* queries, int
                                         int32_t out_type, int64_t out_stride, int64_t max_rows, void* stream);
 /* Waits for `stream` and reports whether a bounded device-side wait of a vx_fp8_scores* call on
  * `device` has run out since the last report (VX_ERR_DEVICE_TIMEOUT; that call's results are
- * incomplete).  The next vx_fp8_scores* call on the device reports it too, without waiting. */
+ * incomplete).  The next vx_fp8_scores* call on the device reports it too, without waiting and without
+ * doing its own work, whichever stream or thread it comes from: the word is one per device, and a wait
+ * that ran out is reported once. */
 VX_API int vx_fp8_check(int32_t device, void* stream);
 
 #ifdef __cplusplus

@@ -296,3 +296,68 @@ def test_first_cuda_call_of_a_thread(call):
         assert torch.equal(out[:n], vx.fp8_scores_device(q[:n], codes, scales))
     elif call == "stored":
         assert torch.equal(out, vx.fp8_scores_device(codes[:300], codes, scales, query_scales=scales[:300]))
+
+
+def test_wait_limit_of_the_hook_is_validated():
+    for limit_ms in (0, 20000):
+        assert N.lib().vx_debug_fp8_wait_timeout(0, limit_ms, None) == N.VX_ERR_INVALID_ARGUMENT
+    assert N.lib().vx_debug_fp8_wait_timeout(-1, 20, None) == N.VX_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.gpu
+def test_a_wait_that_ran_out_is_reported_once():
+    """By fp8_check, or by the next product, which leaves its results as they are; the one after works."""
+    import torch
+
+    q, x = rows_of(3, 100, 1), rows_of(50, 100, 2)
+    codes, scales = _store(x)
+    tq = torch.from_numpy(q).cuda()
+    want = vx.fp8_scores_device(tq, codes, scales)
+    offsets = torch.tensor([0, 3], device="cuda"), torch.tensor([0, 50], device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    vx.fp8_check()
+    assert N.lib().vx_debug_fp8_wait_timeout(0, 20, stream) == 0, N.last_error()
+    with pytest.raises(vx.GpuUnavailableException, match="time budget"):
+        vx.fp8_check()
+    vx.fp8_check()
+    for call in (lambda o: vx.fp8_scores_device(tq, codes, scales, out=o),
+                 lambda o: vx.fp8_scores_grouped_device(tq, offsets[0], codes, scales, offsets[1], out=o)):
+        out = torch.full((3, 50), -7.0, device="cuda")
+        assert N.lib().vx_debug_fp8_wait_timeout(0, 20, stream) == 0
+        torch.cuda.synchronize()
+        with pytest.raises(vx.GpuUnavailableException, match="time budget"):
+            call(out)
+        assert (out == -7).all()
+        assert torch.equal(call(out), want)
+    vx.fp8_check()
+
+
+@pytest.mark.gpu
+def test_a_wait_that_ran_out_is_reported_to_one_of_many_threads():
+    import threading
+
+    import torch
+
+    codes, scales = _store(rows_of(50, 100, 2))
+    q = torch.from_numpy(rows_of(3, 100, 1)).cuda()
+    want = vx.fp8_scores_device(q, codes, scales)
+    for _ in range(20):
+        assert N.lib().vx_debug_fp8_wait_timeout(0, 1, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        start, reports, results = threading.Barrier(8), [], []
+
+        def work():
+            start.wait()
+            try:
+                results.append(vx.fp8_scores_device(q, codes, scales))
+            except vx.GpuUnavailableException as e:
+                reports.append(str(e))
+
+        threads = [threading.Thread(target=work) for _ in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert len(reports) == 1 and "time budget" in reports[0]
+        assert len(results) == 7 and all(torch.equal(r, want) for r in results)

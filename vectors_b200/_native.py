@@ -39,6 +39,7 @@ SIGNATURES = {
     "vx_kernel_launches": [_P],
     "vx_debug_fail_next": [_I32],
     "vx_debug_wait_timeout": [_I32, _I32],
+    "vx_debug_fp8_wait_timeout": [_I32, _I32, _P],
     "vx_profile_enable": [_I32],
     "vx_profile_read": [_I32, _P, _P],
     "vx_profile_reset": [],

@@ -2603,10 +2603,9 @@ int fp8_device(int device, Fp8Device** out) {
   return VX_OK;
 }
 
-// A wait that ran out in an earlier call.
+// A wait that ran out in an earlier call: reported once, by whichever caller takes the word.
 int fp8_pending(Fp8Device* d) {
-  if (*d->err == 0) return VX_OK;
-  *d->err = 0;
+  if (*d->err == 0 || __atomic_exchange_n(d->err, 0, __ATOMIC_ACQ_REL) == 0) return VX_OK;
   return fail(VX_ERR_DEVICE_TIMEOUT, "a device-side wait of an 8-bit score product exceeded its time budget");
 }
 
@@ -2837,6 +2836,18 @@ int vx_fp8_scores_grouped_device(int32_t device, const void* queries, int32_t qu
     if (int s = fp8_check_matrix("out", out, out_type, nq, max_rows, out_stride)) return s;
     return fp8_scores(device, q, codes, scales, n, dim, query_offsets, row_offsets, groups, out, out_type, out_stride,
                       max_rows, (cudaStream_t)stream);
+  });
+}
+
+int vx_debug_fp8_wait_timeout(int32_t device, int32_t timeout_ms, void* stream) {
+  return guarded([&]() -> int {
+    if (timeout_ms < 1 || timeout_ms > 10000)
+      return fail(VX_ERR_INVALID_ARGUMENT, "timeout_ms must be in [1, 10000]: %d", timeout_ms);
+    Fp8Device* dev = nullptr;
+    if (int s = fp8_device(device, &dev)) return s;
+    DeviceScope here(device);
+    VX_LAUNCH(1, launch_wait_probe((uint64_t)timeout_ms * 1000000ull, dev->d_err, (cudaStream_t)stream));
+    return VX_OK;
   });
 }
 
