@@ -361,3 +361,32 @@ def test_a_wait_that_ran_out_is_reported_to_one_of_many_threads():
         torch.cuda.synchronize()
         assert len(reports) == 1 and "time budget" in reports[0]
         assert len(results) == 7 and all(torch.equal(r, want) for r in results)
+
+
+@pytest.mark.gpu
+def test_negated_views():
+    """torch keeps the imaginary part of a conjugate as a view with a flag and the other sign's bits."""
+    import torch
+
+    z = torch.complex(torch.zeros(40, 1), torch.from_numpy(rows_of(40, 1, 1))).cuda()
+    x = z.conj().imag
+    assert x.is_neg()
+    codes, scales = vx.fp8_empty(40, 1)
+    vx.fp8_write_device(x, codes, scales)
+    c, s = encode(x.cpu().numpy())
+    assert np.array_equal(_bytes(codes), c) and np.array_equal(scales.cpu().numpy(), s)
+    d = decode(c, s)
+    got = vx.fp8_scores_device(x, codes, scales)
+    assert (np.abs(got.cpu().numpy() - d @ d.T) <= bound(d, d, "float32")).all()
+    with pytest.raises(vx.IllegalArgumentException, match="negated"):
+        vx.fp8_read_device(codes, scales, 1, out=x)
+
+
+@pytest.mark.gpu
+def test_one_row_broadcast_in_one_dimension():
+    import torch
+
+    x = torch.full((1, 1), 3.25, device="cuda").expand(9, 1)
+    codes, scales = vx.fp8_empty(9, 1)
+    vx.fp8_write_device(x, codes, scales)
+    assert (vx.fp8_read_device(codes, scales, 1) == 3.25).all()

@@ -100,8 +100,9 @@ def _matrix(t, device: int, name: str):
     _on(t, device, name)
     n, dim = t.shape
     step, by = t.stride()
-    if (dim > 1 and by != 1) or (n > 1 and step < dim):
-        t, step = t.contiguous(), dim
+    # negated views (the imaginary part of a conjugate) have steps of two: only single columns need asking
+    if (dim > 1 and by != 1) or (n > 1 and step < dim) or (dim == 1 and t.is_neg()):
+        t, step = t.resolve_neg().contiguous(), dim
     return t, n, dim, step if n > 1 else dim
 
 
@@ -121,6 +122,8 @@ def _out(out, rows: int, columns: int, dtype, codes, zero: bool):
     step, by = out.stride()
     if (columns > 1 and by != 1) or (rows > 1 and step < columns):
         raise IllegalArgumentException("out must have rows of consecutive elements that do not overlap")
+    if columns == 1 and out.is_neg():
+        raise IllegalArgumentException("out must not be a negated view")
     return out, step if rows > 1 else columns
 
 
