@@ -102,6 +102,16 @@ def test_first_row_with_slots(monkeypatch):
     assert "exclude" in message
 
 
+def test_check_of_a_device_that_is_not_there():
+    """The framework's own exceptions, not torch's."""
+    if vx.device_count() == 0:
+        with pytest.raises(vx.GpuUnavailableException):
+            vx.fp8_check()
+    for device in (-1, 63, 64):
+        with pytest.raises((vx.IllegalArgumentException, vx.GpuUnavailableException)):
+            vx.fp8_check(device)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("max_rows", [5, 0])
 def test_no_groups_and_no_offsets(max_rows):

@@ -271,4 +271,6 @@ def fp8_scores_grouped_device(queries, query_offsets, codes, scales, row_offsets
 
 def fp8_check(device: int = 0, stream=None) -> None:
     """Waits for the stream and raises if a bounded wait inside a score product has run out."""
-    _check(_call("vx_fp8_check")(device, _raw_stream(device) if stream is None else stream))
+    if stream is None:  # a device that is not there has no current stream, and the library says so
+        stream = _raw_stream(device) if 0 <= device < torch.cuda.device_count() else 0
+    _check(_call("vx_fp8_check")(device, stream))
