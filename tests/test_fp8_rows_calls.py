@@ -400,3 +400,28 @@ def test_one_row_broadcast_in_one_dimension():
     codes, scales = vx.fp8_empty(9, 1)
     vx.fp8_write_device(x, codes, scales)
     assert (vx.fp8_read_device(codes, scales, 1) == 3.25).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [65536, 65409])
+def test_largest_dimension(dim):
+    """Rows of 512 blocks: written, read back, and scored for float and stored queries, alone and in groups."""
+    import torch
+
+    q, x = rows_of(5, dim, 1, 1.0), rows_of(300, dim, 2, 1.0)
+    tq = torch.from_numpy(q).cuda()
+    codes, scales = vx.fp8_empty(300, dim)
+    vx.fp8_write_device(torch.from_numpy(x).cuda(), codes, scales, slots=torch.arange(299, -1, -1, device="cuda"))
+    c, s = encode(x[::-1])
+    assert np.array_equal(_bytes(codes), c) and np.array_equal(scales.cpu().numpy(), s)
+    dr, dq = decode(c, s), decode(*encode(q))
+    assert np.array_equal(vx.fp8_read_device(codes, scales, dim, first=297).cpu().numpy(), dr[297:, :dim].astype(np.float32))
+    want, tol = dq @ dr.T, bound(dq, dr, "float32")
+    got = vx.fp8_scores_device(tq, codes, scales)
+    assert (np.abs(got.cpu().numpy() - want) <= tol).all()
+    qc, qs = _store(q)
+    assert torch.equal(vx.fp8_scores_device(qc, codes, scales, query_scales=qs), got)
+    assert torch.equal(vx.fp8_scores_device(tq[:1], codes, scales), got[:1])
+    grouped = vx.fp8_scores_grouped_device(tq, torch.tensor([0, 2, 5], device="cuda"), codes, scales,
+                                           torch.tensor([0, 17, 300], device="cuda"), max_rows=283)
+    assert torch.equal(grouped[:2, :17], got[:2, :17]) and torch.equal(grouped[2:], got[2:, 17:])
