@@ -138,11 +138,11 @@ def _slots(slots, device: int):
 
 
 def _place(first: int, n: int, capacity: int, slots) -> None:
-    """Rows first .. first + n - 1 must lie in the store; with slots there is no first row."""
+    """Rows first .. first + n - 1 must lie in the store (the library's check sees 64 bits of a number); with
+    slots there is no first row."""
     if slots is not None:
-        if first != 0:
-            raise IllegalArgumentException(f"first ({first}) and slots exclude each other")
-    elif first < 0 or n > capacity - first:
+        raise IllegalArgumentException(f"first ({first}) and slots exclude each other")
+    if first < 0 or n > capacity - first:
         raise IllegalArgumentException(f"rows [{first}, {first + n}) do not fit a store of {capacity}")
 
 
@@ -170,7 +170,8 @@ def fp8_write_device(rows, codes, scales, slots=None, first: int = 0, stream=Non
         if slots.shape[0] != n:
             raise IllegalArgumentException(f"slots must be [{n}], got {list(slots.shape)}")
         at, size = slots.data_ptr(), slots.element_size()
-    _place(first, n, capacity, slots)
+    if first != 0:
+        _place(first, n, capacity, slots)
     _check(_call("vx_fp8_write_device")(device, rows.data_ptr(), _type_of(rows, "rows"), n, dim, step, at, size, first,
                                         codes.data_ptr(), scales.data_ptr(), capacity, _raw_stream(device)))
 
@@ -194,7 +195,8 @@ def fp8_read_device(codes, scales, dim: int, slots=None, first: int = 0, count: 
         n = capacity - first if count is None else count
     if n < 0 or (count is not None and count != n):
         raise IllegalArgumentException(f"count {count} does not match the {n} rows asked for")
-    _place(first, n, capacity, slots)
+    if first != 0:
+        _place(first, n, capacity, slots)
     out, step = _out(out, n, dim, dtype, codes, False)
     _check(_call("vx_fp8_read_device")(device, codes.data_ptr(), scales.data_ptr(), capacity, dim, at, size, first, n,
                                        out.data_ptr(), _type_of(out, "out"), step, _raw_stream(device)))
