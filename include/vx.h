@@ -355,21 +355,23 @@ VX_API int vx_merge_shards_device(int32_t device, int32_t nshards, const int64_t
  * No counterpart in the reference, whose quantizers are integer or binary.  Rows are kept as e4m3
  * codes with one power-of-two scale for each block of 128 dimensions, in two device buffers that
  * the caller owns (and may slice by rows, save or copy):
- *   codes  [capacity][code_pitch]   e4m3; code_pitch = dim rounded up to 128, columns >= dim zero;
- *                                   16-byte aligned
+ *   codes  [capacity][code_pitch]   e4m3; code_pitch = dim rounded up to 128, columns >= dim zero (0x7f
+ *                                   in a block that is NaN); 16-byte aligned
  *   scales [capacity][scale_pitch]  byte b of block j = 2^(b - 127), 255 = NaN; scale_pitch =
  *                                   code_pitch / 128 rounded up to 4; 4-byte aligned
  * (vx_fp8_pitch gives both).  A block's exponent is the smallest e >= -127 with max |x| <= 448 * 2^e
  * and a code the nearest e4m3 value of x / 2^e, ties to even: |error| <= 2^-4 |x| or 2^-10 * 2^e,
  * whichever is larger.  A block with a NaN or an infinity becomes NaN throughout.  dim <= 65536,
  * capacity < 2^31.  Buffers are device memory of `device`; calls are queued on `stream`, allocate only
- * stream-ordered scratch and can be captured into a graph.  Calls on one store that write and read the
+ * stream-ordered scratch (and, the first of them on a device, one pinned word of host memory) and can be
+ * captured into a graph.  Calls on one store that write and read the
  * same rows must be ordered by the caller (one stream, or events). */
 VX_API int vx_fp8_pitch(int32_t dim, int32_t* code_pitch, int32_t* scale_pitch);
 /* Quantises rows [n][dim] (type VX_F32 / VX_F16 / VX_BF16, row_stride elements apart) into the store:
  * row i goes to slots[i] (slot_bytes 4 or 8: int32 or int64), or to first + i when slots is NULL
  * (first + n <= capacity).  A slot outside [0, capacity) skips its row; where rows of a call name the
- * same slot, the last of them is kept.  Other slots are left as they are. */
+ * same slot, the last of them is kept.  Other slots are left as they are.  A call of more than 512 rows with
+ * slots takes 4 bytes of scratch per slot of the store. */
 VX_API int vx_fp8_write_device(int32_t device, const void* rows, int32_t type, int64_t n, int32_t dim,
                                int64_t row_stride, const void* slots, int32_t slot_bytes, int64_t first,
                                uint8_t* codes, uint8_t* scales, int64_t capacity, void* stream);
@@ -384,9 +386,10 @@ VX_API int vx_fp8_read_device(int32_t device, const uint8_t* codes, const uint8_
  * out_stride elements apart, out_type VX_F32 / VX_F16 / VX_BF16.  Queries [nq][dim] of VX_F32 / VX_F16 /
  * VX_BF16, query_stride elements apart, are quantised as vx_fp8_write_device does; or they are stored
  * rows: query_type VX_E4M3 with their codes and query_scales (query_stride is not used).  Products are
- * exact and summed in fp32 in one order (a query and a row give the same bits in every call; a result
- * whose partial sums leave fp32's range is not finite); a NaN block makes its query's or row's results
- * NaN. */
+ * exact and summed in fp32 by the tensor cores in one order (a query and a row give the same bits in every
+ * call): |error| <= K * 2^-23 * sum |q_k r_k| over the K = code_pitch terms, and 2^-126 where terms fall
+ * below fp32's normal range; a result whose partial sums leave fp32's range is not finite; a NaN block makes
+ * its query's or row's results NaN. */
 VX_API int vx_fp8_scores_device(int32_t device, const void* queries, int32_t query_type, const uint8_t* query_scales,
                                 int64_t nq, int64_t query_stride, const uint8_t* codes, const uint8_t* scales,
                                 int64_t n, int32_t dim, void* out, int32_t out_type, int64_t out_stride, void* stream);

@@ -2,11 +2,12 @@
 //
 // Stored form of a row x: blocks of 128 dimensions, each with one scale 2^e, e the smallest
 // integer >= -127 with max |x| <= 448 * 2^e (448 is e4m3's largest value), kept as the byte
-// e + 127; each element as the nearest e4m3 value of x / 2^e, ties to even.  A power of two costs
-// no accuracy against an arbitrary scale (e4m3 has its own exponent: |error| <= 2^-4 |x|, or
-// 2^-10 * 2^e for elements below 2^-6 * 2^e), the scaling itself is exact, a scale takes one
-// byte, and the tensor cores apply it inside the product (fp8_scores.cu).  A block that holds a
-// NaN or an infinity is NaN throughout: scale byte 255, codes 0x7f.
+// e + 127; each element as the nearest e4m3 value of x / 2^e, ties to even: |error| <= 2^-4 |x|, or
+// 2^-10 * 2^e for elements below 2^-6 * 2^e.  For the larger elements a power of two is as good as
+// an arbitrary scale (e4m3 has its own exponent); it may be up to twice that scale, so the small
+// elements' absolute error may be up to twice what it would be.  In return the scaling itself is exact, a
+// scale takes one byte, and the tensor cores apply it inside the product (fp8_scores.cu).  A block that
+// holds a NaN or an infinity is NaN throughout: scale byte 255, codes 0x7f (past dim too).
 //
 // Both kernels stream: per row they move dim elements and pitch(dim) codes + scales.
 //   write  8 lanes take a block, 16 elements each in pieces of 16 (or 8) bytes, so that both sides are

@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < kTileSlots; s++) {
       mbar_init(&nfull[s], 1);    // the leader's tile warp
-      mbar_init(&nempty[s], 16);  // a stored tile has been read by every role before: the epilogue warps
+      mbar_init(&nempty[s], 16);  // the epilogue warps: a tile that is stored has gone through every role
     }
     mbar_init(drained, 1);
     mbar_init(encoded, 16);  // the epilogue warps of both CTAs
@@ -277,7 +277,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   // The launch before this one wrote the encoded queries, the groups' tile counts and the counter of
   // tiles: every role waits for it before it needs them, and before a bounded wait that would take it
-  // in.  Stored rows and their scales are loaded without it, as far as there is room.
+  // in.  Without groups, stored rows and their scales are loaded without it, as far as there is room; that
+  // helps after a small preparation only, since a cluster starts when one that fills the device has left
+  // two SMs free.
   const bool grouped = a.groups.row_off != nullptr;
   bool waited = !a.wait_first;
   auto wait_for_prep = [&]() {

@@ -243,8 +243,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // The same without ordering this thread's memory accesses before it: for hand-overs that carry no
-// data (TMEM that has been read).  The release at cluster scope above waits for the SM's memory
-// traffic: about 2,000 cycles under load.
+// data (TMEM that has been read, between tcgen05 fences; a tile's description whose values are in
+// use).  The release at cluster scope above waits for the SM's memory traffic: about 2,000 cycles
+// under load.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
