@@ -425,3 +425,57 @@ def test_largest_dimension(dim):
     grouped = vx.fp8_scores_grouped_device(tq, torch.tensor([0, 2, 5], device="cuda"), codes, scales,
                                            torch.tensor([0, 17, 300], device="cuda"), max_rows=283)
     assert torch.equal(grouped[:2, :17], got[:2, :17]) and torch.equal(grouped[2:], got[2:, 17:])
+
+
+@pytest.mark.gpu
+def test_writes_and_products_of_many_threads():
+    """Four threads, each on its stream, mixing writes to slots, reads and all forms of products: clusters of one
+    call start on processors that another's are just leaving.  Every result has the bits of the same call alone."""
+    import threading
+
+    import torch
+
+    r = np.random.default_rng(3)
+    n, dim = 3000, 300
+    x, q = torch.from_numpy(rows_of(n, dim, 1)).cuda(), torch.from_numpy(rows_of(200, dim, 2)).cuda()
+    codes, scales = vx.fp8_empty(n, dim)
+    vx.fp8_write_device(x, codes, scales)
+    slots = torch.from_numpy(r.permutation(n + 500)[:n]).cuda()
+    qo = torch.from_numpy(np.sort(np.concatenate([[0, 200], r.integers(0, 201, 29)]))).cuda()
+    ro = torch.from_numpy(np.sort(np.concatenate([[0, n], r.integers(0, n + 1, 29)]))).cuda()
+
+    def write():
+        c, s = vx.fp8_empty(n + 500, dim)
+        vx.fp8_write_device(x, c, s, slots=slots)
+        return c.view(torch.uint8), s
+
+    calls = [write, lambda: (vx.fp8_read_device(codes, scales, dim, slots=slots),),
+             lambda: (vx.fp8_scores_device(q[:2], codes, scales),), lambda: (vx.fp8_scores_device(q, codes, scales),),
+             lambda: (vx.fp8_scores_device(codes[:50], codes, scales, query_scales=scales[:50]),),
+             lambda: (vx.fp8_scores_grouped_device(q, qo, codes, scales, ro, max_rows=n),)]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(seed):
+        pick = np.random.default_rng(seed)
+        stream = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(100):
+                    ids = pick.integers(0, len(calls), 20)
+                    got = [calls[i]() for i in ids]
+                    stream.synchronize()
+                    for i, g in zip(ids, got):
+                        if not all(torch.equal(a, b) for a, b in zip(g, want[i])):
+                            failed.append(int(i))
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    vx.fp8_check()
+    assert not failed

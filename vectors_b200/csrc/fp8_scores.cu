@@ -654,6 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, kTmemCols);
+    __syncwarp();
   }
   // Nor does the cluster's barrier wait for asynchronous stores (tiles).  A role that ends in order has seen
   // them all; a CTA that gave up stays for what the other may have sent it until then.
@@ -661,7 +662,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t until = globaltimer_ns() + 2000000ull;
     while (globaltimer_ns() < until) {
     }
+    __syncwarp();
   }
+  cluster_meet();  // a pair frees its tensor memory together: neither CTA ends before both have
 }
 
 template <int kType, bool kResident>

@@ -644,7 +644,9 @@ __global__ void __launch_bounds__(64 + 32 * kEpi, 1)
       tmem_dealloc_pair(tmem_base, TMEM_COLS);
     else
       tmem_dealloc(tmem_base, TMEM_COLS);
+    __syncwarp();
   }
+  if (k2Sm) cluster_meet();  // a pair frees its tensor memory together: neither CTA ends before both have
 }
 
 // Shared memory of one CTA with `stages` ring stages and `epi` epilogue warps.
