@@ -39,7 +39,8 @@
 //
 // Few float queries.  Up to 64 queries of 128 blocks in all are quantised by each cluster for itself, into
 // shared memory in the MMA's layout, where they stay for all its tiles: one launch and no scratch
-// (one query x 10k x 768: 10.8 -> 8.2 us a call; x 100k: 20.7 -> 18.5; 37 x 5,003 x 300: 10.8 -> 10.2).
+// (when it came, one query x 10k x 768: 10.8 -> 8.2 us a call; x 100k: 20.7 -> 18.5; 37 x 5,003 x 300:
+// 10.8 -> 10.2; x 100k is 19.2 since the CTAs meet before they allocate).
 //
 // Warps: 0 rows by TMA, 1 TMEM and (leader CTA) MMA, 2 row scales, 3-4 query scales, 5 hand-over of
 // scales, 6 queries by TMA, 7 (leader CTA) tiles, 8-15 epilogue (two per TMEM lane quarter, taking
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
+  cluster_arrive();
   const int64_t unit = blockIdx.x >> 1, units = gridDim.x >> 1;
   if (warp == 0 && lane < 2 && (lane == 0 || !kResident)) prefetch_tmap(lane == 0 ? &maps.rows[0] : &maps.queries[0]);
 
@@ -267,11 +269,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 0;
     fence_mbar_init();
   }
+  // A pair's tensor memory is allocated by both CTAs together, so not before both have started: an
+  // allocation that one began alone, on a busy device, could wait for good.
+  __syncwarp();
+  cluster_wait();
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, kTmemCols);
     tmem_relinquish_pair();
   }
   tc_fence_before();
+  __syncwarp();
   cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;

@@ -317,6 +317,9 @@ __global__ void __launch_bounds__(64 + 32 * kEpi, 1)
   const int64_t p0 = total * unit / units;
   const int64_t p1 = total * (unit + 1) / units;
 
+  // A pair's tensor memory is allocated by both CTAs together, so not before both have started: an
+  // allocation that one began alone, on a busy device, could wait for good.
+  if (k2Sm) cluster_meet();
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stages; s++) {
       mbar_init(&full[s], 1);
